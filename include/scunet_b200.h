@@ -52,7 +52,9 @@ enum {
   SCB_EDEVICE = -5    /* a kernel reported a failure through the device error word */
 };
 
-enum { SCB_F32 = 0, SCB_U8 = 1 };
+/* Element types. Images are SCB_F32 or SCB_U8; the block operators at the end of this
+ * header take SCB_F32, SCB_F16 and SCB_BF16 tensors and integer or float positions. */
+enum { SCB_F32 = 0, SCB_U8 = 1, SCB_F16 = 2, SCB_BF16 = 3, SCB_I32 = 4, SCB_I64 = 5 };
 
 /* Validate, repack (fp16 K-major tiles) and upload every weight once.
  * Replaces `Cuda::new(&Weights)` (src/cuda.rs:192-241). `config` is the seven
@@ -298,6 +300,80 @@ int scb_profile_kernels(const scb_ctx* ctx, char* buf, size_t cap);
  * TFLOP/s, class). Writes at most cap - 1 bytes and a NUL into buf (buf may be NULL
  * to size it); returns the full length. Empty when profiling is off. */
 int scb_profile_report(scb_ctx* ctx, char* buf, size_t cap);
+
+/* ---------------------------------------------------------------------------------------
+ * Block operators: what image and video U-Net blocks use beside this network's own - group
+ * norm with an activation, rotation of queries and keys by position axes, attention over
+ * all tokens of a map. The reference has none of them.
+ *
+ * They take no context: device pointers of the current device, element strides, the
+ * caller's workspace (16-byte aligned, at least the bytes its _workspace call gives, used
+ * by one call at a time) and a stream (NULL: the default stream). They are asynchronous,
+ * allocate nothing and can be captured in a CUDA graph. Inputs may overlap one another
+ * (stride 0 broadcasts), outputs may not, except as stated. On failure the message is in
+ * scb_last_error (NULL) of the calling thread, and nothing was launched.
+ * ------------------------------------------------------------------------------------- */
+enum { SCB_ACT_NONE = 0, SCB_ACT_RELU = 1, SCB_ACT_GELU = 2, SCB_ACT_SILU = 3 };
+
+int scb_group_norm_workspace(int64_t n, int64_t l, int c, int groups, size_t* bytes);
+
+/* y = act((x - mean) / sqrt(var + eps) * weight + bias), channels last: x is n pictures of
+ * l rows (pixels) of c contiguous channels, pictures x_sn and rows x_sl elements apart; mean
+ * and (biased) variance are those of a picture's group of c / groups channels. weight and
+ * bias are float32 [c] or NULL (1 and 0). y may be x. mean and rstd (1 / sqrt(var + eps)),
+ * float32 [n][groups], are written where not NULL: scb_group_norm_backward wants them.
+ * Statistics are float32 joins of shifted partial sums; GELU is the exact (erf) form. A
+ * picture of no rows gives mean 0 and rstd 1 / sqrt(eps). */
+int scb_group_norm(const void* x, int64_t x_sn, int64_t x_sl, int dtype, int64_t n, int64_t l, int c, int groups,
+                   const float* weight, const float* bias, float eps, int act, void* y, int64_t y_sn, int64_t y_sl,
+                   float* mean, float* rstd, void* work, size_t work_bytes, void* stream);
+
+/* The gradient: dx (may be dy or x), and where not NULL dweight and dbias (float32 [c],
+ * overwritten), from dy, the forward's x and its mean and rstd. ReLU's slope at 0 is 0. */
+int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const void* x, int64_t x_sn, int64_t x_sl,
+                            int dtype, int64_t n, int64_t l, int c, int groups, const float* mean, const float* rstd,
+                            const float* weight, const float* bias, int act, void* dx, int64_t dx_sn, int64_t dx_sl,
+                            float* dweight, float* dbias, void* work, size_t work_bytes, void* stream);
+
+/* One operand of scb_rotate_axes: [b][l][heads][d], the d channels contiguous, the other
+ * element strides given. y may be x. */
+typedef struct {
+  const void* x;
+  void* y;
+  int heads;
+  int64_t x_sb, x_sl, x_sh, y_sb, y_sl, y_sh;
+} scb_heads;
+
+enum { SCB_ROT_HALF = 0, SCB_ROT_INTERLEAVED = 1, SCB_ROT_AXIAL = 2 };
+
+/* Rotates the channel pairs of queries and keys (k may be NULL) by the token's position on
+ * 1 to 4 axes. sections[a] pairs turn with axis a, in order, P in all (2 P <= d); channels
+ * past 2 P are copied. Pair p turns by t = pos[token][a(p)] * inv_freq[p] (one float32
+ * product): (u, v) -> (u cos t - v sin t, u sin t + v cos t), by -t with `inverse`, which is
+ * also the gradient. Channels (u, v) of pair p: SCB_ROT_HALF p and p + P;
+ * SCB_ROT_INTERLEAVED 2 p and 2 p + 1; SCB_ROT_AXIAL halves of each axis's own 2 sections[a]
+ * channels. pos is [b][l][axes] by its element strides (pos_sb 0: the same for every
+ * picture), SCB_I32, SCB_I64 or SCB_F32; inv_freq is float32 [P]; sections is on the host. */
+int scb_rotate_axes(const scb_heads* q, const scb_heads* k, int dtype, int64_t b, int64_t l, int d, const void* pos,
+                    int pos_dtype, int64_t pos_sb, int64_t pos_sl, int64_t pos_sa, const float* inv_freq,
+                    const int* sections, int axes, int layout, int inverse, void* stream);
+
+/* [b][l][heads][d] by its element strides, the d channels contiguous. */
+typedef struct {
+  void* x;
+  int64_t sb, sl, sh;
+} scb_rows;
+
+int scb_attention_workspace(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, size_t* bytes);
+
+/* o = softmax(scale q k^T over the visible keys) v for q, o [b][lq][h][d] and k, v
+ * [b][lk][hk][d] in SCB_F16 or SCB_BF16, d at most 256; query head i reads key head
+ * i / (h / hk). key_mask (NULL: all visible) is bytes [b][lk], rows mask_sb apart, 0 =
+ * hidden: a hidden key's values do not matter, NaN and infinities included. Queries with no
+ * visible key give zeros. */
+int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const scb_rows* o, int dtype, int64_t b,
+                  int64_t lq, int64_t lk, int h, int hk, int d, const unsigned char* key_mask, int64_t mask_sb,
+                  float scale, void* work, size_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,7 +23,7 @@ from . import plan as _plan
 HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libscunet_b200.so"
 
-SCB_F32, SCB_U8 = 0, 1
+SCB_F32, SCB_U8, SCB_F16, SCB_BF16, SCB_I32, SCB_I64 = range(6)
 SYMBOLS = [
     "scb_create", "scb_forward", "scb_forward_dev", "scb_forward_host", "scb_need_bytes", "scb_footprint",
     "scb_release_scratch", "scb_last_error", "scb_destroy", "scb_probe_gemm", "scb_probe_conv3x3",
@@ -32,6 +32,8 @@ SYMBOLS = [
     "scb_forward_bands", "scb_band_unique_id", "scb_band_init", "scb_forward_band", "scb_profile_bytes", "scb_probe_mlp",
     "scb_band_sync", "scb_probe_head", "scb_probe_tail", "scb_probe_wait_timeout", "scb_mem_report",
     "scb_profile_report", "scb_check_admission", "scb_profile_kernels",
+    "scb_group_norm_workspace", "scb_group_norm", "scb_group_norm_backward", "scb_rotate_axes",
+    "scb_attention_workspace", "scb_attention",
 ]
 SCB_OPT_FUSE_TRANS = 1
 SCB_OPT_RESIDUAL32 = 2
@@ -44,6 +46,10 @@ OP_CLASSES = ["head", "tail", "conv1x1", "conv3x3", "qkv", "attention", "proj", 
               "trans_fused", "halo", "mlp"]
 
 
+SCB_ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+SCB_ROT_LAYOUTS = {"half": 0, "interleaved": 1, "axial": 2}
+
+
 class BackendError(RuntimeError):
     pass
 
@@ -51,6 +57,15 @@ class BackendError(RuntimeError):
 class ScbTensor(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("data", ctypes.POINTER(ctypes.c_float)), ("ndim", ctypes.c_int),
                 ("shape", ctypes.c_int64 * 4)]
+
+
+class ScbHeads(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("heads", ctypes.c_int)] + [
+        (f, ctypes.c_int64) for f in ("x_sb", "x_sl", "x_sh", "y_sb", "y_sl", "y_sh")]
+
+
+class ScbRows(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("sb", ctypes.c_int64), ("sl", ctypes.c_int64), ("sh", ctypes.c_int64)]
 
 
 _lib = None
@@ -107,6 +122,14 @@ def load_library(path=None):
     lib.scb_set_option.argtypes = [vp, i, i]
     lib.scb_profile_read.argtypes = [vp, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_double),
                                      ctypes.POINTER(ctypes.c_float), i]
+    i64, f32, heads, rows = ctypes.c_int64, ctypes.c_float, ctypes.POINTER(ScbHeads), ctypes.POINTER(ScbRows)
+    lib.scb_group_norm_workspace.argtypes = [i64, i64, i, i, ctypes.POINTER(sz)]
+    lib.scb_group_norm.argtypes = [vp, i64, i64, i, i64, i64, i, i, vp, vp, f32, i, vp, i64, i64, vp, vp, vp, sz, vp]
+    lib.scb_group_norm_backward.argtypes = [vp, i64, i64, vp, i64, i64, i, i64, i64, i, i, vp, vp, vp, vp, i, vp, i64,
+                                            i64, vp, vp, vp, sz, vp]
+    lib.scb_rotate_axes.argtypes = [heads, heads, i, i64, i64, i, vp, i, i64, i64, i64, vp, vp, i, i, i, vp]
+    lib.scb_attention_workspace.argtypes = [i64, i64, i64, i, i, i, ctypes.POINTER(sz)]
+    lib.scb_attention.argtypes = [rows, rows, rows, rows, i, i64, i64, i64, i, i, i, vp, i64, f32, vp, sz, vp]
     if path is None:
         _lib = lib
     return lib

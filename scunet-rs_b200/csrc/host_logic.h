@@ -10,10 +10,39 @@
 //    hang.
 #pragma once
 #include <cstddef>
+#include <cstdint>
 #include <cstdio>
 #include <string>
 
 namespace scb {
+
+// Keeps the message of a failed call that has no context for scb_last_error(NULL) on this
+// thread and returns `code` (defined beside scb_last_error).
+int global_error(int code, const std::string& msg);
+
+// Whether no two elements of a strided output coincide: `inner` contiguous elements, then
+// dimensions of `size` elements `stride` apart, in any order.
+struct Dim {
+  int64_t size, stride;
+};
+template <size_t N>
+bool distinct_elements(int64_t inner, const Dim (&given)[N]) {
+  Dim d[N];
+  for (size_t i = 0; i < N; ++i) d[i] = given[i];
+  for (size_t i = 1; i < N; ++i)  // insertion sort by stride
+    for (size_t j = i; j > 0 && d[j].stride < d[j - 1].stride; --j) {
+      const Dim t = d[j];
+      d[j] = d[j - 1];
+      d[j - 1] = t;
+    }
+  int64_t extent = inner;
+  for (size_t i = 0; i < N; ++i) {
+    if (d[i].size <= 1) continue;
+    if (d[i].stride < extent) return false;
+    extent += (d[i].size - 1) * d[i].stride;
+  }
+  return true;
+}
 
 enum class Admit { ok, refuse, unknown_free };
 

@@ -13,9 +13,10 @@
 namespace scb {
 
 // Device-wide error word: 0 = ok; otherwise the first failure's code (see
-// SCB_ERR_* below). Read and cleared by the host after every forward. The library
-// is one translation unit, so this header is included exactly once.
-__device__ unsigned int g_device_error = 0;
+// SCB_ERR_* below). Each of the library's two translation units (the network and the
+// block operators) has its own: the host reads and clears the network's after every
+// forward, the operators' in scb_op_status.
+static __device__ unsigned int g_device_error = 0;
 
 enum : unsigned {
   SCB_ERR_WAIT_FULL = 1,   // MMA waited for a TMA stage that never landed

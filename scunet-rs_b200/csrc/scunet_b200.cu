@@ -794,6 +794,12 @@ int fail(scb_ctx* ctx, int code, const std::string& msg) {
   return code;
 }
 
+}  // namespace
+
+int scb::global_error(int code, const std::string& msg) { return fail(nullptr, code, msg); }
+
+namespace {
+
 int cuda_fail(scb_ctx* ctx, cudaError_t e, const char* what) {
   return fail(ctx, SCB_ECUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }

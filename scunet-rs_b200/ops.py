@@ -1,0 +1,269 @@
+"""Block operators on torch CUDA tensors, over the context-free entries of
+`include/scunet_b200.h`: what image and video U-Net blocks use beside the network's own.
+
+  group_norm, group_norm_backward   group norm with an activation, channels last
+  rotate_axes                       queries and keys rotated by time / row / column
+  attention                         attention over all tokens of a map, with a key mask
+
+Every call runs on the current stream of its tensors' device, takes its outputs and its
+workspace from torch's caching allocator (so a workspace lives as long as the stream needs
+it) and returns before the GPU has finished. Inputs may be views: only the channels have to
+be contiguous. `GroupNormAct` and `RotateAxes` are the same for autograd. Wrong arguments
+raise `BackendError`; there is no fallback for tensors that are not on a CUDA device.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .backend import (SCB_ACTS, SCB_BF16, SCB_F16, SCB_F32, SCB_I32, SCB_I64, SCB_ROT_LAYOUTS, BackendError, ScbHeads,
+                      ScbRows, load_library)
+
+_DTYPES = {torch.float32: SCB_F32, torch.float16: SCB_F16, torch.bfloat16: SCB_BF16}
+_POSITIONS = {torch.int32: SCB_I32, torch.int64: SCB_I64, torch.float32: SCB_F32}
+
+
+def _fail(msg):
+    raise BackendError(msg)
+
+
+def _check(rc, lib):
+    if rc != 0:
+        raise BackendError(lib.scb_last_error(None).decode())
+
+
+def _dtype(t, what):
+    if not t.is_cuda:
+        _fail(f"{what} must be on a CUDA device")
+    if t.dtype not in _DTYPES:
+        _fail(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _same(t, like, what):
+    if t.dtype != like.dtype or t.device != like.device or t.shape != like.shape:
+        _fail(f"{what} must be {tuple(like.shape)} {like.dtype} on {like.device}, "
+              f"not {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _params(t, c, like, what):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.device != like.device or t.shape != (c,) or not t.is_contiguous():
+        _fail(f"{what} must be {c} contiguous float32 values on {like.device}")
+    return t.data_ptr()
+
+
+def _rows(t, what):
+    """(pictures, rows, channels, picture stride, row stride) of [n][...][c]; the dimensions
+    between collapse to rows of one stride."""
+    if t.dim() < 2:
+        _fail(f"{what} must be [pictures, ..., channels]")
+    shape, stride = t.shape, t.stride()
+    if shape[-1] > 1 and stride[-1] != 1:
+        _fail(f"{what}: the channels must be contiguous (channels last)")
+    rows, sl = 1, 0
+    for size, st in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
+        if size == 1:
+            continue
+        if rows > 1 and st != sl * rows:
+            _fail(f"{what}: the dimensions between pictures and channels must have one common row stride")
+        if rows == 1:
+            sl = st
+        rows *= size
+    return shape[0], rows, shape[-1], stride[0], sl
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _workspace(fn, lib, device, *sizes):
+    need = ctypes.c_size_t(0)
+    _check(fn(*sizes, ctypes.byref(need)), lib)
+    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act="none", out=None, stats=False):
+    """act((x - mean) / sqrt(var + eps) * weight + bias) of x [n, ..., c], channels last.
+
+    Mean and variance are those of each picture's c / groups neighbouring channels; weight
+    and bias are float32 [c]; act is "none", "relu", "gelu" (exact) or "silu". `out` may be x.
+    With stats=True also returns mean and 1 / sqrt(var + eps), float32 [n, groups]."""
+    dt = _dtype(x, "x")
+    n, l, c, sn, sl = _rows(x, "x")
+    if act not in SCB_ACTS:
+        _fail(f"unknown activation {act!r}")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _same(out, x, "out")
+    _, _, _, on, ol = _rows(out, "out")
+    w, b = _params(weight, c, x, "weight"), _params(bias, c, x, "bias")
+    lib = load_library()
+    with torch.cuda.device(x.device):
+        mean = rstd = None
+        if stats:
+            mean, rstd = (torch.empty((n, max(groups, 1)), dtype=torch.float32, device=x.device) for _ in range(2))
+        work = _workspace(lib.scb_group_norm_workspace, lib, x.device, n, l, c, groups)
+        _check(lib.scb_group_norm(x.data_ptr(), sn, sl, dt, n, l, c, groups, w, b, eps, SCB_ACTS[act], out.data_ptr(),
+                                  on, ol, _ptr(mean), _ptr(rstd), _ptr(work), work.numel() if n else 0, _stream(x)), lib)
+    return (out, mean, rstd) if stats else out
+
+
+def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, act="none", out=None):
+    """(dx, dweight, dbias) of group_norm from dy, its x and its mean and rstd (stats=True).
+    dweight and dbias are float32 [c] whether or not weight and bias are given; `out` (dx) may
+    be dy or x."""
+    dt = _dtype(x, "x")
+    n, l, c, sn, sl = _rows(x, "x")
+    _same(dy, x, "dy")
+    _, _, _, dn, dl = _rows(dy, "dy")
+    if act not in SCB_ACTS:
+        _fail(f"unknown activation {act!r}")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _same(out, x, "out")
+    _, _, _, on, ol = _rows(out, "out")
+    w, b = _params(weight, c, x, "weight"), _params(bias, c, x, "bias")
+    for t, what in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype != torch.float32 or t.device != x.device or t.shape != (n, groups) or not t.is_contiguous():
+            _fail(f"{what} must be contiguous float32 [{n}, {groups}] on {x.device}")
+    lib = load_library()
+    with torch.cuda.device(x.device):
+        dw, db = (torch.empty(c, dtype=torch.float32, device=x.device) for _ in range(2))
+        work = _workspace(lib.scb_group_norm_workspace, lib, x.device, n, l, c, groups)
+        _check(lib.scb_group_norm_backward(dy.data_ptr(), dn, dl, x.data_ptr(), sn, sl, dt, n, l, c, groups,
+                                           mean.data_ptr(), rstd.data_ptr(), w, b, SCB_ACTS[act], out.data_ptr(), on,
+                                           ol, dw.data_ptr(), db.data_ptr(), _ptr(work), work.numel() if n else 0,
+                                           _stream(x)), lib)
+    return out, dw, db
+
+
+def _heads(x, out, what):
+    if x.dim() != 4:
+        _fail(f"{what} must be [pictures, tokens, heads, channels]")
+    if x.shape[3] > 1 and (x.stride(3) != 1 or out.stride(3) != 1):
+        _fail(f"{what}: the channels must be contiguous")
+    return ScbHeads(x.data_ptr(), out.data_ptr(), x.shape[2], *x.stride()[:3], *out.stride()[:3])
+
+
+def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=False, out=None):
+    """(q, k) rotated by their tokens' positions on 1 to 4 axes (k may be None).
+
+    q is [b, l, h, d], k [b, l, hk, d]; positions [l, axes] or [b, l, axes], int32, int64 or
+    float32; inv_freq float32 [sum(sections)]: sections[a] channel pairs turn by
+    positions[..., a] * inv_freq. layout: "half" pairs channels (p, p + P), "interleaved"
+    (2p, 2p + 1), "axial" the halves of each axis's own channels; channels past 2 P are
+    copied. inverse=True turns back, which is the gradient. `out` is a pair of tensors, which
+    may be (q, k) themselves."""
+    dt = _dtype(q, "q")
+    if layout not in SCB_ROT_LAYOUTS:
+        _fail(f"unknown layout {layout!r}")
+    if q.dim() != 4:
+        _fail("q must be [pictures, tokens, heads, channels]")
+    b, l, _, d = q.shape
+    if k is not None and (k.dtype != q.dtype or k.device != q.device or k.dim() != 4 or k.shape[:2] != (b, l)
+                          or k.shape[3] != d):
+        _fail(f"k must be [{b}, {l}, heads, {d}] {q.dtype} on {q.device}")
+    axes = len(sections)
+    if positions.dtype not in _POSITIONS or positions.device != q.device:
+        _fail(f"positions must be int32, int64 or float32 on {q.device}")
+    if positions.shape == (l, axes):
+        pb, (pl, pa) = 0, positions.stride()
+    elif positions.shape == (b, l, axes):
+        pb, pl, pa = positions.stride()
+    else:
+        _fail(f"positions must be [{l}, {axes}] or [{b}, {l}, {axes}], not {tuple(positions.shape)}")
+    _params(inv_freq, sum(sections), q, "inv_freq")
+    if out is None:
+        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+               None if k is None else torch.empty(k.shape, dtype=k.dtype, device=q.device))
+    _same(out[0], q, "out[0]")
+    qh, kh = _heads(q, out[0], "q"), None
+    if k is not None:
+        _same(out[1], k, "out[1]")
+        kh = _heads(k, out[1], "k")
+    lib = load_library()
+    with torch.cuda.device(q.device):
+        _check(lib.scb_rotate_axes(qh, kh, dt, b, l, d, positions.data_ptr(), _POSITIONS[positions.dtype], pb, pl, pa,
+                                   inv_freq.data_ptr(), (ctypes.c_int * axes)(*sections), axes,
+                                   SCB_ROT_LAYOUTS[layout], bool(inverse), _stream(q)), lib)
+    return out
+
+
+def attention(q, k, v, *, scale=None, key_mask=None, out=None):
+    """softmax(scale q k^T over the visible keys) v, float16 or bfloat16.
+
+    q is [b, lq, h, d], k and v [b, lk, hk, d] with d at most 256; query head i reads key head
+    i / (h / hk). key_mask is bool or uint8 [b, lk], nonzero = visible: what hidden keys hold
+    does not matter, and queries with no visible key give zeros. scale defaults to
+    1 / sqrt(d)."""
+    dt = _dtype(q, "q")
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4 or t.dtype != q.dtype or t.device != q.device:
+            _fail(f"{what} must be [pictures, tokens, heads, channels] {q.dtype} on {q.device}")
+        if t.shape[3] > 1 and t.stride(3) != 1:
+            _fail(f"{what}: the channels must be contiguous")
+    b, lq, h, d = q.shape
+    _, lk, hk, _ = k.shape
+    if k.shape != (b, lk, hk, d) or v.shape != k.shape:
+        _fail(f"k and v must be [{b}, keys, heads, {d}] alike, not {tuple(k.shape)} and {tuple(v.shape)}")
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.device != q.device \
+                or key_mask.shape != (b, lk) or (lk > 1 and key_mask.stride(1) != 1):
+            _fail(f"key_mask must be bool or uint8 [{b}, {lk}] on {q.device}, its rows contiguous")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _same(out, q, "out")
+        if d > 1 and out.stride(3) != 1:
+            _fail("out: the channels must be contiguous")
+    lib = load_library()
+    with torch.cuda.device(q.device):
+        work = _workspace(lib.scb_attention_workspace, lib, q.device, b, lq, lk, h, hk, d)
+        rows = [ScbRows(t.data_ptr(), *t.stride()[:3]) for t in (q, k, v, out)]
+        _check(lib.scb_attention(*rows, dt, b, lq, lk, h, hk, d, _ptr(key_mask),
+                                 0 if key_mask is None else key_mask.stride(0), d ** -0.5 if scale is None else scale,
+                                 _ptr(work), 0 if work is None else work.numel(), _stream(q)), lib)
+    return out
+
+
+class GroupNormAct(torch.autograd.Function):
+    """group_norm under autograd: GroupNormAct.apply(x, groups, weight, bias, eps, act)."""
+
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, eps=1e-5, act="none"):
+        y, mean, rstd = group_norm(x, groups, weight, bias, eps=eps, act=act, stats=True)
+        ctx.save_for_backward(x, mean, rstd, weight, bias)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, mean, rstd, weight, bias = ctx.saved_tensors
+        dy = dy.contiguous()  # a gradient may come broadcast
+        dx, dw, db = group_norm_backward(dy, x, mean, rstd, ctx.groups, weight, bias, act=ctx.act)
+        return dx, None, dw if weight is not None else None, db if bias is not None else None, None, None
+
+
+class RotateAxes(torch.autograd.Function):
+    """rotate_axes under autograd: RotateAxes.apply(q, k, positions, inv_freq, sections, layout)."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, sections, layout="half"):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.sections, ctx.layout = tuple(sections), layout
+        return rotate_axes(q, k, positions, inv_freq, sections, layout=layout)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, inv_freq = ctx.saved_tensors
+        dq, dk = rotate_axes(dq.contiguous(), dk.contiguous(), positions, inv_freq, ctx.sections, layout=ctx.layout, inverse=True)
+        return dq, dk, None, None, None, None
