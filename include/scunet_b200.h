@@ -375,6 +375,10 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
                   int64_t lq, int64_t lk, int h, int hk, int d, const unsigned char* key_mask, int64_t mask_sb,
                   float scale, void* work, size_t work_bytes, void* stream);
 
+/* Waits for `stream` and reports a block operator that gave up on a bounded device wait
+ * (SCB_EDEVICE; its outputs are undefined) since the last call on this device. */
+int scb_op_status(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <initializer_list>
@@ -12,6 +13,7 @@
 #include "../../include/scunet_b200.h"
 #include "host_logic.h"
 #include "op_attn.cuh"
+#include "op_attn_tc.cuh"
 #include "op_norm.cuh"
 #include "op_rotary.cuh"
 
@@ -146,6 +148,98 @@ void norm_backward(const NormGeom& g, const void* dy, const void* x, void* dx, c
     norm_backward_act<T, V, ACT_SILU>(g, dy, x, dx, mean, rstd, w, b, dw, db, part, sums, st);
   else
     norm_backward_act<T, V, ACT_NONE>(g, dy, x, dx, mean, rstd, w, b, dw, db, part, sums, st);
+}
+
+// ---------------------------------------------------------------------------- attention
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+    return reinterpret_cast<EncodeTiledFn>(e == cudaSuccess && q == cudaDriverEntryPointSuccess ? p : nullptr);
+  }();
+  return fn;
+}
+
+// K or V as [picture][head][key][channel]: boxes of 128 keys x 64 channels, 128-byte
+// swizzle; channels past d and keys past lk read zeros. A dimension that is broadcast
+// (stride 0) or single has extent 1.
+bool attn_map(CUtensorMap* m, const scb_rows& t, int dtype, int64_t b, int64_t lk, int hk, int d) {
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const bool hs = hk > 1 && t.sh, bs = b > 1 && t.sb;
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)lk, (cuuint64_t)(hs ? hk : 1), (cuuint64_t)(bs ? b : 1)};
+  cuuint64_t strides[3] = {lk > 1 ? (cuuint64_t)t.sl * 2 : 16, hs ? (cuuint64_t)t.sh * 2 : 16,
+                           bs ? (cuuint64_t)t.sb * 2 : 16};
+  cuuint32_t box[4] = {64, AT_KEYS, 1, 1}, one[4] = {1, 1, 1, 1};
+  return fn(m, dtype == SCB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.x, dims,
+            strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Whether TMA can read the tensor: 16-byte aligned rows, strides in its range.
+bool attn_tma_ok(const scb_rows& t, int64_t b, int64_t lk, int hk) {
+  const int64_t most = 1ll << 38;  // elements: strides below 2^40 bytes, with room
+  if (addr(t.x) % 16 || lk > 0x7fffff00) return false;
+  if (lk > 1 && (t.sl <= 0 || t.sl % 8 || t.sl > most)) return false;
+  if (hk > 1 && (t.sh % 8 || t.sh > most)) return false;
+  return !(b > 1 && (t.sb % 8 || t.sb > most));
+}
+
+// How the tensor-core kernel cuts the work (op_attn_tc.cuh).
+struct AttnPlan {
+  int twin, unit_rows, share;
+  long rows, row_units, units, tiles, total;
+  int grid;
+  bool cut;
+  size_t work;
+};
+AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int sms) {
+  AttnPlan p{};
+  p.share = h / hk;
+  p.rows = lq * p.share;
+  p.tiles = (lk + AT_KEYS - 1) / AT_KEYS;
+  p.twin = p.rows <= 128 && p.tiles > 1;
+  p.unit_rows = p.twin ? 128 : 256;
+  p.row_units = (p.rows + p.unit_rows - 1) / p.unit_rows;
+  p.units = b * hk * p.row_units;
+  p.total = p.units * p.tiles;
+  long grid = p.units;
+  const long waves = (p.units + sms - 1) / sms;
+  if (p.units < sms) {
+    const long most = p.total / 4;  // at least four tiles a CTA
+    grid = most < p.units ? p.units : most < sms ? most : sms;
+  } else if (!p.twin && p.units < waves * sms * 95 / 100) {
+    grid = sms;
+  }
+  p.grid = (int)(grid < kMaxBlocks ? grid : kMaxBlocks);
+  p.cut = p.grid != p.units;
+  p.work = p.cut || p.twin ? (size_t)p.grid * 2 * 256 * (d + 2) * sizeof(float) : 0;
+  return p;
+}
+
+template <typename T, int Boxes>
+int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk, const CUtensorMap& tv,
+                   cudaStream_t st) {
+  const auto kernel = attn_tc_kernel<T, Boxes>;
+  constexpr int smem = AtLayout<Boxes>::kSmem;
+  // the kernel's shared memory limit is raised once on each device
+  static std::atomic<uint64_t> raised{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(raised.load() & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
+    raised.fetch_or(bit);
+  }
+  kernel<<<p.grid, AT_THREADS, smem, st>>>(tk, tv, g);
+  if (p.cut || p.twin) attn_join_kernel<T><<<(unsigned)((p.units * p.unit_rows + 3) / 4), 128, 0, st>>>(g, p.grid);
+  return launched("scb_attention");
 }
 
 // f<T, V>() for the element type and vector width.
@@ -326,6 +420,10 @@ int scb_attention_workspace(int64_t b, int64_t lq, int64_t lk, int h, int hk, in
     *bytes = 0;
     if (b < 0 || lq < 0 || lk < 0 || h < 1 || hk < 1 || h % hk || d < 1)
       return refuse("scb_attention_workspace", "bad sizes");
+    if (!b || !lq || !lk || d > 128) return SCB_OK;
+    const int sms = sm_count();
+    if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
+    *bytes = attn_plan(b, lq, lk, h, hk, d, sms).work;
     return SCB_OK;
   });
 }
@@ -350,8 +448,6 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
     }
     if (!distinct_elements(d, {{b, o->sb}, {lq, o->sl}, {h, o->sh}})) return refuse(op, "overlapping output");
     if (key_mask && mask_sb < 0) return refuse(op, "negative strides");
-    (void)work;
-    (void)work_bytes;
     AttnArgs a{};
     a.q = q->x; a.k = k->x; a.v = v->x; a.o = o->x;
     a.mask = key_mask; a.m_sb = mask_sb;
@@ -362,6 +458,37 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
     a.o_sb = o->sb; a.o_sl = o->sl; a.o_sh = o->sh;
     a.scale_log2 = scale * 1.4426950408889634f;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (lk && d <= 128 && attn_tma_ok(*k, b, lk, hk) && attn_tma_ok(*v, b, lk, hk)) {
+      const int sms = sm_count();
+      if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
+      const AttnPlan p = attn_plan(b, lq, lk, h, hk, d, sms);
+      if (p.units <= kMaxBlocks / 256) {
+        if (p.work && (!work || work_bytes < p.work || addr(work) % 16))
+          return refuse(op, "the workspace is too small or not 16-byte aligned (scb_attention_workspace)");
+        AttnTcArgs g{};
+        g.a = a;
+        g.share = p.share; g.rows = p.rows; g.twin = p.twin; g.unit_rows = p.unit_rows; g.row_units = p.row_units;
+        g.units = p.units; g.tiles = p.tiles; g.total = p.total;
+        g.kv_b = (b > 1 && k->sb ? 1 : 0) | (b > 1 && v->sb ? 2 : 0);
+        g.kv_h = (hk > 1 && k->sh ? 1 : 0) | (hk > 1 && v->sh ? 2 : 0);
+        g.qneg = scale < 0 ? 1 : a.scale_log2 == 0 ? 2 : 0;
+        g.a.scale_log2 = g.qneg == 2 ? 1.f : std::fabs(a.scale_log2);
+        g.part = static_cast<float*>(work);
+        g.part_ml = reinterpret_cast<float2*>(g.part + (size_t)p.grid * 2 * 256 * d);
+        const auto wide = [&](const scb_rows* t) {
+          return addr(t->x) % 16 == 0 && t->sb % 8 == 0 && t->sl % 8 == 0 && t->sh % 8 == 0;
+        };
+        g.q_wide = wide(q);
+        g.o_wide = wide(o);
+        CUtensorMap tk, tv;
+        if (!attn_map(&tk, *k, dtype, b, lk, hk, d) || !attn_map(&tv, *v, dtype, b, lk, hk, d))
+          return global_error(SCB_ECUDA, "scb_attention: no tensor map for k or v");
+        if (dtype == SCB_F16)
+          return d <= 64 ? attn_tc_launch<__half, 1>(g, p, tk, tv, st) : attn_tc_launch<__half, 2>(g, p, tk, tv, st);
+        return d <= 64 ? attn_tc_launch<__nv_bfloat16, 1>(g, p, tk, tv, st)
+                       : attn_tc_launch<__nv_bfloat16, 2>(g, p, tk, tv, st);
+      }
+    }
     const long blocks = (lq + ATTN_ANY_WARPS - 1) / ATTN_ANY_WARPS;
     if (b > kMaxBlocks / h || blocks > kMaxBlocks / (b * h)) return refuse(op, "too many queries");
     if (dtype == SCB_F16)
@@ -369,6 +496,20 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
     else
       attn_any_kernel<__nv_bfloat16><<<(unsigned)(blocks * b * h), 32 * ATTN_ANY_WARPS, 0, st>>>(a);
     return launched(op);
+  });
+}
+
+int scb_op_status(void* stream) {
+  return guarded([&]() -> int {
+    cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+    unsigned v = 0;
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof v);
+    if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_op_status: ") + cudaGetErrorString(e));
+    if (!v) return SCB_OK;
+    const unsigned zero = 0;
+    cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
+    return global_error(SCB_EDEVICE,
+                        "a kernel gave up on a bounded wait (device error code " + std::to_string(v) + ")");
   });
 }
 

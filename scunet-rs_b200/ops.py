@@ -4,6 +4,7 @@
   group_norm, group_norm_backward   group norm with an activation, channels last
   rotate_axes                       queries and keys rotated by time / row / column
   attention                         attention over all tokens of a map, with a key mask
+  status                            wait, and raise if a kernel gave up on a device wait
 
 Every call runs on the current stream of its tensors' device, takes its outputs and its
 workspace from torch's caching allocator (so a workspace lives as long as the stream needs
@@ -233,6 +234,15 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
                                  0 if key_mask is None else key_mask.stride(0), d ** -0.5 if scale is None else scale,
                                  _ptr(work), 0 if work is None else work.numel(), _stream(q)), lib)
     return out
+
+
+def status(stream=None):
+    """Wait for the stream (default: the current one) and raise if an operator's kernel gave up
+    on a bounded wait since the last call; its outputs are undefined then."""
+    stream = stream or torch.cuda.current_stream()
+    with torch.cuda.device(stream.device):
+        lib = load_library()
+        _check(lib.scb_op_status(stream.cuda_stream), lib)
 
 
 class GroupNormAct(torch.autograd.Function):
