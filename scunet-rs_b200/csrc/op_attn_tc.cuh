@@ -11,13 +11,16 @@
 // once; of a unit that is cut, every piece goes to the workspace as float32 sums with its
 // maximum and total, and attn_join_kernel adds them in order (no atomics).
 //
-// CTA: warps 0-3 and 4-7 are the softmax of tile 0 and 1, one thread a row; warp 8 issues
-// the matrix products, warp 9 the TMA loads of K and V into a ring of 128-key slots (warps
-// 10 and 11 fill their warpgroup up, which gives registers to the softmax).
+// CTA: warps 0-7 and 8-15 are the softmax of tile 0 and 1, two threads a row with 64 keys
+// each; warps 16 and 17 issue the matrix products of tile 0 and 1, warp 18 the TMA loads of
+// K and V into a ring of 128-key slots (warp 19 fills the warpgroup up, which gives
+// registers to the softmax).
 //   S_t = Q_t K^T    M 128, N 128, K d        TMEM columns [128 t, +128)
-//   P_t = 2^(c S - c m), 16-bit               columns [128 t, +64), over S
-//   O_t += P_t V     M 128, N d, K 128        columns [256 + 128 t, +d), A from TMEM
-// While one tile's softmax runs, the tensor cores compute the other tile's products. The
+//   P_t = 2^(c S - c m), 16-bit               64 columns
+//   O_t += P_t V     M 128, N d, K 128        columns [256 + 64 or 128 t, +d), A from TMEM
+// Heads up to 64 wide leave columns for P_t beside S_t, so the next S_t is computed as soon
+// as this one is in registers; with wider heads P_t lies over S_t and the next S_t waits
+// for P_t V. While one tile's softmax runs, the tensor cores compute the other tile's products. The
 // maximum m that a row subtracts is raised only when a tile exceeds it by 2^8 (in P): sums
 // are float32 and P at most 256, so a stale m changes no result, and O, which lives in
 // TMEM, is rescaled only then.
@@ -27,9 +30,13 @@
 namespace scb {
 
 constexpr int AT_KEYS = 128;               // keys of a tile
-constexpr int AT_THREADS = 384;            // launched with 168 registers a thread
+constexpr int AT_THREADS = 640;            // launched with 96 registers a thread
 constexpr float AT_STALE = 8.f;            // log2 by which a tile may exceed m
 constexpr int AT_BOX = AT_KEYS * 128;      // bytes of 128 rows x 64 channels
+
+// Of every 16 pairs of weights, those whose 2^y is computed by exp2_pair on the FMA units
+// instead of the special function unit.
+constexpr int AT_FMA_PAIRS = 2;
 
 struct AttnTcArgs {
   AttnArgs a;
@@ -42,7 +49,7 @@ struct AttnTcArgs {
   long total;         // units * tiles
   int kv_b, kv_h;     // 1 where K / V differ by picture / head (0: broadcast), bit 0 K, bit 1 V
   int qneg;           // the scale is negative (Q is negated) or, 2, zero (Q is cleared)
-  float* part;        // pieces: [grid][2][256][d] sums, then [grid][2][256] (m c, l)
+  float* part;        // pieces: [grid][2][d][256] sums, then [grid][2][256] (m c, l)
   float2* part_ml;
   int q_wide, o_wide; // 16-byte accesses to Q and the output allowed
 };
@@ -63,6 +70,49 @@ __device__ __forceinline__ uint32_t at_pack<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// 2^y of two values y <= 8 on the FMA units: y = n + f, n the nearest integer (it appears in
+// the low bits of y + 1.5 2^23), |f| <= 1/2; 2^f by the cubic of least relative error on that
+// interval (fitted by linear programming: 7.5e-5 at most, 5.2e-5 rms, where rounding the
+// weight to fp16 adds 2e-4 rms and to bf16 1.6e-3), then n is added to the exponent. Below
+// y = -126 the result stays at 2^-126; NaN gives NaN or the largest float, which at_total
+// finds in the sum.
+__device__ __forceinline__ float2 exp2_pair(float2 y) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.y) : "f"(-126.f));
+  const float2 z = __fadd2_rn(y, make_float2(12582912.f, 12582912.f));
+  const float2 n = __fadd2_rn(z, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), y);
+  float2 p = __ffma2_rn(f, make_float2(0.0551714189f, 0.0551714189f), make_float2(0.24261117f, 0.24261117f));
+  p = __ffma2_rn(p, f, make_float2(0.693261027f, 0.693261027f));
+  p = __ffma2_rn(p, f, make_float2(0.999928057f, 0.999928057f));
+  // p + (z << 23) as one multiply-add
+  int rx, ry;
+  asm("mad.lo.s32 %0, %1, 8388608, %2;" : "=r"(rx) : "r"(__float_as_int(z.x)), "r"(__float_as_int(p.x)));
+  asm("mad.lo.s32 %0, %1, 8388608, %2;" : "=r"(ry) : "r"(__float_as_int(z.y)), "r"(__float_as_int(p.y)));
+  return make_float2(__int_as_float(rx), __int_as_float(ry));
+}
+
+// A sum of weights as it is, or NaN when a weight was (weights are at most 2^8, so a sum of
+// them stays far below 1e30).
+__device__ __forceinline__ float at_total(float l) { return l < 1e30f ? l : NAN; }
+
+// Whether `p` holds for any of the 256 threads of barrier `id`, which all arrive.
+__device__ __forceinline__ bool at_any(int id, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"((uint32_t)p)
+      : "memory");
+  return r != 0;
+}
+// The two tiles' exponentials take turns: a tile waits for its turn, and gives the other
+// tile's half-way through its own (512 threads: 256 wait, 256 give).
+__device__ __forceinline__ void at_turn_wait(int t) { asm volatile("barrier.cta.sync %0, 512;" ::"r"(3 + t) : "memory"); }
+__device__ __forceinline__ void at_turn_give(int t) { asm volatile("barrier.cta.arrive %0, 512;" ::"r"(4 - t) : "memory"); }
+__device__ __forceinline__ void at_sync(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
+
 // Boxes: 64-channel halves of a head (1 or 2); Slots: K and V tiles in the ring.
 template <int Boxes>
 struct AtLayout {
@@ -71,8 +121,23 @@ struct AtLayout {
   static constexpr int kQ = 0;
   static constexpr int kRing = 2 * kTile;
   static constexpr int kBars = kRing + kSlots * kTile;
-  static constexpr int kSmem = kBars + 256 + 1024;        // + alignment to 1 KB
+  // full and empty of every slot, six pairs of barriers, the TMEM address, `dead`
+  static constexpr int kRow = kBars + 8 * (2 * kSlots + 12) + 8;  // [2 tiles][2 halves][128] floats
+  static constexpr int kSmem = kRow + 2048;
+  // TMEM columns: S_t at 128 t; then O_t, and P_t where there is room for it
+  static constexpr bool kOwnP = Boxes == 1;
+  static constexpr int kO = 256, kOStep = 64 * Boxes;
+  static constexpr int kP = kOwnP ? 384 : 0, kPStep = kOwnP ? 64 : 128;
 };
+
+// One lane of a converged warp. Selecting the issuing thread this way instead of by lane
+// number lets the compiler keep descriptors in uniform registers: eight products were
+// issued in 780 cycles before.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 
 // A bounded wait that gives up at once when another wait of the CTA has given up.
 __device__ __forceinline__ void at_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
@@ -86,34 +151,35 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                const __grid_constant__ AttnTcArgs g) {
   using L = AtLayout<Boxes>;
-  extern __shared__ uint8_t at_raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(at_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t sm[];  // the swizzled tiles' alignment
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::kBars);
   uint64_t* empty = full + L::kSlots;
   uint64_t* q_ready = empty + L::kSlots;
   uint64_t* s_full = q_ready + 2;
   uint64_t* p_ready = s_full + 2;
   uint64_t* o_done = p_ready + 2;
-  uint64_t* drain = o_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* s_free = o_done + 2;
+  uint64_t* drain = s_free + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < L::kSlots; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, 1);
+      mbar_init(empty + i, g.twin ? 1 : 2);  // the tiles that read the slot
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(q_ready + t, 128);
+      mbar_init(q_ready + t, 256);
       mbar_init(s_full + t, 1);
-      mbar_init(p_ready + t, 128);
+      mbar_init(p_ready + t, 256);
       mbar_init(o_done + t, 1);
+      mbar_init(s_free + t, 256);
+      mbar_init(drain + t, 1);
     }
-    mbar_init(drain, 1);
     *dead = 0;
     mbar_fence_init();
   }
-  if (warp == 8) tmem_alloc(tmem_slot, 512);
+  if (warp == 16) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -121,10 +187,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   const long x0 = at_start(g, blockIdx.x, gridDim.x), x1 = at_start(g, blockIdx.x + 1, gridDim.x);
   const int d = g.a.d, ksteps = (d + 15) / 16;
 
-  // 384 x 168 = 64512 registers at launch; 256 x 208 + 128 x 80 = 63488 after the two splits
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == 9 && lane == 0) {
+  // 640 x 96 = 61440 registers at launch, 512 x 104 + 128 x 64 = 61440 after the split
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == 18 && elect_one()) {
       // ---- TMA: K and V tiles into the ring, in the order of their use
       uint32_t seq = 0;
       for (long x = x0; x < x1;) {
@@ -149,101 +215,120 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           const uint32_t s = seq - back;
           mbar_wait(full + s % L::kSlots, (s / L::kSlots) & 1, SCB_ERR_WAIT_ATTN);
         }
-    } else if (warp == 8 && lane == 0) {
-      // ---- matrix products
+    } else if (warp < 18 && elect_one()) {
+      // ---- matrix products of tile t
+      const int t = warp - 16;
       const uint32_t sb = smem_u32(sm);
-      constexpr bool kBf = sizeof(T) == 2 && !__is_same(T, __half);
-      constexpr uint32_t fmt = kBf ? (1u << 7) | (1u << 10) : 0u;
-      const uint32_t id_s = make_idesc_f16(128, 128) | fmt;
+      constexpr uint32_t fmt = __is_same(T, __half) ? 0u : (1u << 7) | (1u << 10);  // bf16 operands
+      constexpr uint32_t id_s = make_idesc_f16(128, 128) | fmt;
       const uint32_t id_o = make_idesc_f16_bmn(128, 16 * ksteps) | fmt;
-      uint32_t cnt[2] = {0, 0}, segs[2] = {0, 0}, base = 0;
-      auto scores = [&](int t, uint32_t jj, bool release) {
-        const uint32_t seq = 2 * jj, slot = seq % L::kSlots;
+      const uint64_t dq = make_sdesc(sb + L::kQ + t * L::kTile, 128, SW_128B);
+      const uint64_t dk = make_sdesc(sb + L::kRing, 128, SW_128B);
+      const uint64_t dv = make_sdesc_lbo_sbo(sb + L::kRing, AT_BOX, 1024, SW_128B);
+      const uint32_t ts = tmem + 128 * t, tp = tmem + L::kP + L::kPStep * t, to = tmem + L::kO + L::kOStep * t;
+      const uint32_t step = g.twin ? 4 : 2;  // ring places from one K to the tile's next
+      uint32_t cnt = 0, segs = 0, base = 0;
+      const auto scores = [&](uint32_t seq) {
+        const uint32_t slot = seq % L::kSlots;
         at_wait(full + slot, (seq / L::kSlots) & 1, dead);
         tc_fence_after();
-        const uint32_t q = sb + L::kQ + t * L::kTile, k = sb + L::kRing + slot * L::kTile;
-        for (int s = 0; s < ksteps; ++s) {
-          const uint32_t o = (s >> 2) * AT_BOX + (s & 3) * 32;
-          umma_f16(tmem + 128 * t, make_sdesc(q + o, 128, SW_128B), make_sdesc(k + o, 128, SW_128B), id_s, s > 0);
+        const uint64_t k = dk + slot * (uint32_t)(L::kTile >> 4);
+#pragma unroll
+        for (int s = 0; s < 4 * Boxes; ++s) {
+          const uint32_t o = ((s >> 2) * AT_BOX + (s & 3) * 32) >> 4;
+          if (s < ksteps) umma_f16(ts, dq + o, k + o, id_s, s > 0);
         }
         umma_commit(s_full + t);
-        if (release) umma_commit(empty + slot);
+        umma_commit(empty + slot);
       };
       for (long x = x0; x < x1;) {
         const long unit = x / g.tiles, j0 = x - unit * g.tiles;
         const uint32_t n = (uint32_t)min(x1 - x, g.tiles - j0);
-        const uint32_t nt[2] = {g.twin ? (n + 1) / 2 : n, g.twin ? n / 2 : n};
-        for (int t = 0; t < 2; ++t) {
-          if (!nt[t]) continue;
-          at_wait(q_ready + t, segs[t]++ & 1, dead);
+        const uint32_t nt = g.twin ? (n + 1 - t) / 2 : n;
+        uint32_t seq = 2 * (base + (g.twin ? t : 0));  // of K; V is the next
+        if (nt) {
+          at_wait(q_ready + t, segs++ & 1, dead);
           tc_fence_after();
-          scores(t, base + (g.twin ? t : 0), g.twin || t == 1);
+          scores(seq);
         }
-        for (uint32_t i = 0; i < nt[0]; ++i)
-          for (int t = 0; t < 2; ++t) {
-            if (i >= nt[t]) continue;
-            const uint32_t jj = base + (g.twin ? 2 * i + t : i);
-            at_wait(p_ready + t, cnt[t] & 1, dead);
-            const uint32_t seq = 2 * jj + 1, slot = seq % L::kSlots;
-            at_wait(full + slot, (seq / L::kSlots) & 1, dead);
-            tc_fence_after();
-            const uint32_t v = sb + L::kRing + slot * L::kTile;
-#pragma unroll
-            for (int s = 0; s < AT_KEYS / 16; ++s)
-              umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * s,
-                          make_sdesc_lbo_sbo(v + 2048 * s, AT_BOX, 1024, SW_128B), id_o, i > 0 || s > 0);
-            umma_commit(o_done + t);
-            if (g.twin || t == 1) umma_commit(empty + slot);
-            if (i + 1 < nt[t]) {
-              // S_t overwrites P_t, so P_t V must have read it; the other tile's softmax
-              // runs meanwhile
-              at_wait(o_done + t, cnt[t] & 1, dead);
-              scores(t, base + (g.twin ? 2 * (i + 1) + t : i + 1), g.twin || t == 1);
-            }
-            ++cnt[t];
-            if (*dead) break;
+        for (uint32_t i = 0; i < nt && !*dead; ++i, ++cnt, seq += step) {
+          if (L::kOwnP && i + 1 < nt) {  // the next scores, as soon as S_t is in registers
+            at_wait(s_free + t, cnt & 1, dead);
+            scores(seq + step);
           }
+          const uint32_t slot = (seq + 1) % L::kSlots;
+          at_wait(full + slot, ((seq + 1) / L::kSlots) & 1, dead);
+          const uint64_t v = dv + slot * (uint32_t)(L::kTile >> 4);
+          at_wait(p_ready + t, cnt & 1, dead);
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < AT_KEYS / 16; ++s)
+            umma_f16_ts(to, tp + 8 * s, v + (uint32_t)(2048 * s >> 4), id_o, i > 0 || s > 0);
+          umma_commit(o_done + t);
+          umma_commit(empty + slot);
+          if (!L::kOwnP && i + 1 < nt) {
+            // S_t overwrites P_t, so P_t V must have read it; the other tile's softmax runs
+            // meanwhile
+            at_wait(o_done + t, cnt & 1, dead);
+            scores(seq + step);
+          }
+        }
         base += n;
         x += n;
       }
       if (*dead) {  // products may still be running on TMEM and shared memory
-        umma_commit(drain);
-        mbar_wait(drain, 0, SCB_ERR_WAIT_ATTN);
+        umma_commit(drain + t);
+        mbar_wait(drain + t, 0, SCB_ERR_WAIT_ATTN);
       }
     }
   } else {
-    // ---- softmax: tile t, one thread a row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int t = warp >> 2, row = tid & 127;
+    // ---- softmax: tile t, two threads a row (warps 8 t + w and 8 t + 4 + w)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int t = warp >> 3, half = warp >> 2 & 1, row = tid & 127, id = 1 + t;
     const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = trow + 128 * t, to = trow + 256 + 128 * t;
+    const uint32_t ts = trow + 128 * t + 64 * half, to = trow + L::kO + L::kOStep * t;
+    const uint32_t tp = trow + L::kP + L::kPStep * t + 32 * half;
     uint8_t* sq = sm + L::kQ + t * L::kTile;
+    float* mine = reinterpret_cast<float*>(sm + L::kRow) + 256 * t + 128 * half + row;
+    const float* other = reinterpret_cast<float*>(sm + L::kRow) + 256 * t + 128 * (half ^ 1) + row;
     const float c = g.a.scale_log2, stale = fminf(AT_STALE / c, 1e30f);
+    const int last = (int)(g.tiles - 1), tail = (int)(g.a.lk - (long)last * AT_KEYS) - 64 * half;  // of the last tile, past this half's first key
     uint32_t cnt = 0, base = 0;
+    if (t == 1) at_turn_give(t);
     for (long x = x0; x < x1;) {
       const long unit = x / g.tiles, j0 = x - unit * g.tiles, n = min(x1 - x, g.tiles - j0);
       const long bh = unit / g.row_units;
       const int b = (int)(bh / g.a.hk), hk = (int)(bh - (long)b * g.a.hk);
       const long r = (unit - bh * g.row_units) * g.unit_rows + (g.twin ? 0 : 128 * t) + row;
-      const bool on = r < g.rows;
-      const long ql = on ? r / g.share : 0;
-      const int qh = hk * g.share + (int)(on ? r - ql * g.share : 0);
-      const long step = g.twin ? 2 : 1, jt = j0 + (g.twin ? t : 0);
-      const bool any = jt < j0 + n;
+      const int step = g.twin ? 2 : 1, jt = (int)j0 + (g.twin ? t : 0), jn = (int)(j0 + n);
+      const bool any = jt < jn;
+      // row rr of this warp's 32 (or -1 past the last): its query and head
+      const int warp_row = (warp & 3) * 32;
+      const long r0 = r - lane;
+      const auto locate = [&](int rr, int64_t sb, int64_t sl, int64_t sh) -> long {
+        const long x = r0 + rr;
+        if (x >= g.rows) return -1;
+        const long at = g.share == 1 ? x : x / g.share;
+        return b * sb + at * sl + (hk * g.share + (x - at * g.share)) * sh;
+      };
+      const int chunks = 2 * ksteps, wide = chunks > 8 ? 16 : chunks > 4 ? 8 : 4;  // 16-byte chunks of a row
       if (any) {
-        // this row of Q, zeros past the last row and channel; K-major, 128-byte swizzle
-        const T* q = static_cast<const T*>(g.a.q) + b * g.a.q_sb + ql * g.a.q_sl + qh * g.a.q_sh;
+        // this warp's 16 rows of Q, `wide` lanes a row; zeros past the last row and channel.
+        // K-major, 128-byte swizzle
         const uint32_t flip = g.qneg == 1 ? 0x80008000u : 0u;
-        for (int k = 0; k < 2 * ksteps; ++k) {
+        const int k = lane & (wide - 1);
+        for (int rr = 16 * half + lane / wide; rr < 16 * half + 16; rr += 32 / wide) {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (on && g.qneg < 2) {
+          const long at = locate(rr, g.a.q_sb, g.a.q_sl, g.a.q_sh);
+          if (at >= 0 && g.qneg < 2 && k < chunks) {
+            const T* q = static_cast<const T*>(g.a.q) + at + 8 * k;
             if (g.q_wide && 8 * k + 8 <= d) {
-              v = *reinterpret_cast<const uint4*>(q + 8 * k);
+              v = *reinterpret_cast<const uint4*>(q);
             } else {
               const unsigned short* e = reinterpret_cast<const unsigned short*>(q);
               unsigned w[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) w[i] = 8 * k + i < d ? e[8 * k + i] : 0;
+              for (int i = 0; i < 8; ++i) w[i] = 8 * k + i < d ? e[i] : 0;
               v = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
             }
             v.x ^= flip;
@@ -251,68 +336,89 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             v.z ^= flip;
             v.w ^= flip;
           }
-          *reinterpret_cast<uint4*>(sq + (k >> 3) * AT_BOX + swz_off(row, k & 7, 128)) = v;
+          if (k < chunks) *reinterpret_cast<uint4*>(sq + (k >> 3) * AT_BOX + swz_off(warp_row + rr, k & 7, 128)) = v;
         }
         fence_proxy_async_smem();
         mbar_arrive(q_ready + t);
       }
       const unsigned char* mask = g.a.mask ? g.a.mask + b * g.a.m_sb : nullptr;
       float m = -INFINITY, l = 0.f;
-      for (long j = jt; j < j0 + n; j += step) {
-        // which keys of the tile are visible, one bit each
-        uint32_t seen[4];
-        {
-          const long key = j * AT_KEYS + lane;
+      const uint32_t first = cnt;
+      unsigned char ahead[2] = {1, 1};  // the next tile's mask bytes, 0 past the last key
+      const auto look = [&](int j) {
+        if (!mask || j > last) return;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const long k = key + 32 * i;
-            seen[i] = __ballot_sync(0xffffffffu, k < g.a.lk && (!mask || mask[k]));
+        for (int i = 0; i < 2; ++i)
+          ahead[i] = j < last || 32 * i + lane < tail ? mask[(long)j * AT_KEYS + 64 * half + 32 * i + lane] : 0;
+      };
+      look(jt);
+      for (int j = jt; j < jn; j += step) {
+        // which of this half's keys are visible, one bit each
+        bool part = !mask && j == last && tail < 64;
+        uint32_t seen[2];
+        if (mask) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) seen[i] = __ballot_sync(0xffffffffu, ahead[i] != 0);
+          part = (seen[0] & seen[1]) != 0xffffffffu;
+          look(j + step);
+        } else if (part) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int k = tail - 32 * i;
+            seen[i] = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
           }
         }
         at_wait(s_full + t, cnt & 1, dead);
         tc_fence_after();
-        float s[128];
+        float s[64];
         {
-          uint32_t u[128];
+          uint32_t u[64];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) tmem_ld16_issue(ts + 16 * i, u + 16 * i);
+          for (int i = 0; i < 4; ++i) tmem_ld16_issue(ts + 16 * i, u + 16 * i);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4; ++i) {
             tmem_fence16(u + 16 * i);
             u32_to_f32_16(u + 16 * i, s + 16 * i);
           }
         }
-        const bool part = (seen[0] & seen[1] & seen[2] & seen[3]) != 0xffffffffu;
+        if (L::kOwnP) {
+          tc_fence_before();
+          mbar_arrive(s_free + t);
+        }
         if (part) {
+          asm volatile("");  // keeps this a branch: 64 selects would cost every tile
 #pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] = seen[i >> 5] >> (i & 31) & 1 ? s[i] : -INFINITY;
+          for (int i = 0; i < 64; ++i) s[i] = seen[i >> 5] >> (i & 31) & 1 ? s[i] : -INFINITY;
           if (mask) {
-            // hidden values may be NaN or infinite, and 0 times those is NaN: clear them
-            const uint32_t seq = 2 * (base + (uint32_t)(j - j0)) + 1, slot = seq % L::kSlots;
+            // hidden values may be NaN or infinite, and 0 times those is NaN: clear this
+            // half's hidden rows of V, 64 threads each half of a row's chunks or boxes
+            const uint32_t seq = 2 * (base + (uint32_t)(j - (int)j0)) + 1, slot = seq % L::kSlots;
             at_wait(full + slot, (seq / L::kSlots) & 1, dead);
-            const uint32_t word = (row >> 5) == 0 ? seen[0] : (row >> 5) == 1 ? seen[1] : (row >> 5) == 2 ? seen[2] : seen[3];
-            if (!(word >> (row & 31) & 1)) {
-              uint4* v = reinterpret_cast<uint4*>(sm + L::kRing + slot * L::kTile + row * 128);
-              for (int k = 0; k < 8; ++k) {
-                v[k] = make_uint4(0, 0, 0, 0);
-                if (Boxes == 2) v[AT_BOX / 16 + k] = make_uint4(0, 0, 0, 0);
-              }
+            if (!((row & 32 ? seen[1] : seen[0]) >> (row & 31) & 1)) {
+              uint4* v = reinterpret_cast<uint4*>(sm + L::kRing + slot * L::kTile + (64 * half + (row & 63)) * 128 +
+                                                  (row >> 6) * (Boxes == 2 ? AT_BOX : 64));
+              for (int k = 0; k < 4 * Boxes; ++k) v[k] = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
           }
         }
-        const float top = row_max<128>(s);
-        if (j == jt) {
-          m = top;
-        } else {
-          const bool raise = top > m + stale;
-          if (__any_sync(0xffffffffu, raise)) {
-            // P_t V of the tile before is complete (S_t was issued after it)
+        float top = row_max<64>(s);
+        if (cnt > first) at_wait(o_done + t, (cnt - 1) & 1, dead);  // O_t is complete, P_t read
+        // (the barrier also keeps P_t, where it lies over S_t, behind both halves' loads)
+        if (at_any(id, j == jt || top > m + stale)) {
+          *mine = top;
+          at_sync(id);
+          top = fmaxf(top, *other);
+          if (j == jt) {
+            m = top;
+          } else {
+            tc_fence_after();
+            const bool raise = top > m + stale;
             const float f = raise ? ex2_approx((m - top) * c) : 1.f;
             m = raise ? top : m;
-            l *= f;
-            for (int i = 0; i < ksteps; ++i) {
+            l = at_total(l) * f;
+            for (int i = half; i < ksteps; i += 2) {
               float o[16];
               tmem_ld16(to + 16 * i, o);
 #pragma unroll
@@ -321,20 +427,24 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             }
           }
         }
-        const float mc = m == -INFINITY ? 0.f : -m * c;
+        // an infinite score makes the row NaN, as inf - inf would
+        const float mc = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m * c;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        at_turn_wait(t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 y = __ffma2_rn(make_float2(s[32 * i + 2 * e], s[32 * i + 2 * e + 1]), make_float2(c, c),
                                         make_float2(mc, mc));
-            const float2 v = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+            const float2 v = (e * AT_FMA_PAIRS) % 16 < AT_FMA_PAIRS ? exp2_pair(y)
+                                                                    : make_float2(ex2_approx(y.x), ex2_approx(y.y));
             sum[e & 1] = __fadd2_rn(sum[e & 1], v);
             p[e] = at_pack<T>(v.x, v.y);
           }
-          tmem_st16u(ts + 16 * i, p);
+          tmem_st16u(tp + 16 * i, p);
+          if (i == 0) at_turn_give(t);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
@@ -342,93 +452,127 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         mbar_arrive(p_ready + t);
         ++cnt;
       }
+      if (g.twin && t == 1 && n % 2 == 1) {  // tile 0 had one key tile more
+        at_turn_wait(t);
+        at_turn_give(t);
+      }
       // ---- the unit's rows: to the output when the unit is whole, else to the workspace
       if (any) {
         at_wait(o_done + t, (cnt - 1) & 1, dead);
         tc_fence_after();
       }
+      *mine = l;
+      at_sync(id);
+      l = at_total(half ? *other + l : l + *other);
       if (!g.twin && n == g.tiles) {
+        // through the Q tile, whose products are complete: 16-byte chunks of whole rows,
+        // `wide` lanes a row, as Q was read
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        T* o = static_cast<T*>(g.a.o) + b * g.a.o_sb + ql * g.a.o_sl + qh * g.a.o_sh;
-        for (int i = 0; i < ksteps; ++i) {
+        for (int i = half; i < ksteps; i += 2) {
           float v[16];
           tmem_ld16(to + 16 * i, v);
-          if (!on) continue;
-          if (g.o_wide && 16 * i + 16 <= d) {
-            uint32_t w[8];
+          uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = at_pack<T>(v[2 * e] * inv, v[2 * e + 1] * inv);
-            *reinterpret_cast<uint4*>(o + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(o + 16 * i + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          for (int e = 0; e < 8; ++e) w[e] = at_pack<T>(v[2 * e] * inv, v[2 * e + 1] * inv);
+          uint8_t* o = sq + (i >> 2) * AT_BOX;
+          *reinterpret_cast<uint4*>(o + swz_off(row, (2 * i) & 7, 128)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(o + swz_off(row, (2 * i + 1) & 7, 128)) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+        at_sync(id);
+        const int k = lane & (wide - 1);
+        for (int rr = 16 * half + lane / wide; rr < 16 * half + 16; rr += 32 / wide) {
+          const long at = locate(rr, g.a.o_sb, g.a.o_sl, g.a.o_sh);
+          if (at < 0 || k >= chunks) continue;
+          const uint4 v = *reinterpret_cast<const uint4*>(sq + (k >> 3) * AT_BOX + swz_off(warp_row + rr, k & 7, 128));
+          T* o = static_cast<T*>(g.a.o) + at + 8 * k;
+          if (g.o_wide && 8 * k + 8 <= d) {
+            *reinterpret_cast<uint4*>(o) = v;
           } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (16 * i + e < d) o[16 * i + e] = from_f32<T>(v[e] * inv);
+            const T* e = reinterpret_cast<const T*>(&v);
+            for (int i = 0; i < 8; ++i)
+              if (8 * k + i < d) o[i] = e[i];
           }
         }
       } else {
-        const long at = (2L * blockIdx.x + (x == x0 ? 0 : 1)) * 256 + 128 * t + row;
-        if (on) g.part_ml[at] = make_float2(m == -INFINITY ? m : m * c, l);
-        float* o = g.part + at * d;
-        for (int i = 0; i < ksteps; ++i) {
+        // the piece is kept channel by channel, so that a warp stores 32 rows side by side
+        const long piece = 2L * blockIdx.x + (x == x0 ? 0 : 1);
+        if (half == 0) g.part_ml[piece * 256 + 128 * t + row] = make_float2(m == -INFINITY ? m : m * c, l);
+        float* o = g.part + piece * 256 * d + 128 * t + row;
+        for (int i = half; i < ksteps; i += 2) {
           float v[16];
           if (any) tmem_ld16(to + 16 * i, v);
-          if (!on) continue;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (16 * i + e < d) o[16 * i + e] = any ? v[e] : 0.f;
+            if (16 * i + e < d) o[(16 * i + e) * 256] = any ? v[e] : 0.f;
         }
       }
       tc_fence_before();
+      at_sync(id);  // the Q tile and the rows' sums are written again
       base += (uint32_t)n;
       x += n;
     }
+    if (t == 0) at_turn_wait(t);  // the other tile's last
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
-// Adds the pieces of the units that were cut: one warp a row.
+// Adds the pieces of the units that were cut, 32 rows a block:
 //   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, M the largest m_i
+// A lane is a row (the pieces are stored channel by channel); the result goes through
+// shared memory to be written row by row.
+constexpr int AT_JOIN = 256;
 template <typename T>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnTcArgs g, int grid) {
-  const int lane = threadIdx.x & 31, d = g.a.d;
-  const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const long unit = w / g.unit_rows;
-  const int row = (int)(w - unit * g.unit_rows);
-  if (unit >= g.units) return;
-  const long bh = unit / g.row_units, r = (unit - bh * g.row_units) * g.unit_rows + row;
-  if (r >= g.rows) return;
+__global__ void __launch_bounds__(AT_JOIN) attn_join_kernel(const __grid_constant__ AttnTcArgs g, int grid) {
+  __shared__ T out[32][130];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = g.a.d;
+  const int groups = g.unit_rows / 32;
+  const long unit = blockIdx.x / groups;
+  const int row = (int)(blockIdx.x - unit * groups) * 32 + lane;
+  const long bh = unit / g.row_units, r0 = (unit - bh * g.row_units) * g.unit_rows + row - lane;
+  if (r0 >= g.rows) return;
   const long t0 = unit * g.tiles, c0 = at_owner(g, t0, grid), c1 = at_owner(g, t0 + g.tiles - 1, grid);
   if (c0 == c1 && !g.twin) return;  // written by its CTA
   const int subs = g.twin ? 2 : 1;
   const int pieces = (int)(c1 - c0 + 1) * subs;
-  auto place = [&](int i) {
+  const auto piece = [&](int i) {
     const long cta = c0 + i / subs;
-    return (2 * cta + (at_start(g, cta, grid) >= t0 ? 0 : 1)) * 256 + row + 128 * (i % subs);
+    return 2 * cta + (at_start(g, cta, grid) >= t0 ? 0 : 1);
   };
   float top = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, g.part_ml[place(i)].x);
-  for (int k = 16; k >= 1; k /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+  for (int i = 0; i < pieces; ++i) top = fmaxf(top, g.part_ml[piece(i) * 256 + 128 * (i % subs) + row].x);
+  constexpr int kMost = 128 / (AT_JOIN / 32);  // channels of a warp
+  float o[kMost], l = 0.f;
+#pragma unroll
+  for (int k = 0; k < kMost; ++k) o[k] = 0.f;
   for (int i = 0; i < pieces; ++i) {
-    const long at = place(i);
-    const float2 ml = g.part_ml[at];
+    const long p = piece(i);
+    const int col = 128 * (i % subs) + row;
+    const float2 ml = g.part_ml[p * 256 + col];
     const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
     l += f * ml.y;
+    const float* part = g.part + p * 256 * d + col;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane + 32 * k < d && f != 0.f) o[k] += f * g.part[at * d + lane + 32 * k];
+    for (int k = 0; k < kMost; ++k)
+      if (warp + k * (AT_JOIN / 32) < d) {
+        const float v = part[(warp + k * (AT_JOIN / 32)) * 256];
+        o[k] += f == 0.f ? 0.f : f * v;
+      }
   }
-  const int b = (int)(bh / g.a.hk), hk = (int)(bh - (long)b * g.a.hk);
-  const long ql = r / g.share;
-  const int qh = hk * g.share + (int)(r - ql * g.share);
-  T* out = static_cast<T*>(g.a.o) + b * g.a.o_sb + ql * g.a.o_sl + qh * g.a.o_sh;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 32 * k < d) out[lane + 32 * k] = from_f32<T>(l == 0.f ? 0.f : o[k] / l);
+  for (int k = 0; k < kMost; ++k)
+    if (warp + k * (AT_JOIN / 32) < d) out[lane][warp + k * (AT_JOIN / 32)] = from_f32<T>(o[k] * inv);
+  __syncthreads();
+  const int b = (int)(bh / g.a.hk), hk = (int)(bh - (long)b * g.a.hk);
+  for (int rr = warp; rr < 32 && r0 + rr < g.rows; rr += AT_JOIN / 32) {
+    const long ql = (r0 + rr) / g.share;
+    const long qh = hk * g.share + (r0 + rr - ql * g.share);
+    T* dst = static_cast<T*>(g.a.o) + b * g.a.o_sb + ql * g.a.o_sl + qh * g.a.o_sh;
+    for (int c = lane; c < d; c += 32) dst[c] = out[rr][c];
+  }
 }
 
 }  // namespace scb

@@ -238,7 +238,7 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
     raised.fetch_or(bit);
   }
   kernel<<<p.grid, AT_THREADS, smem, st>>>(tk, tv, g);
-  if (p.cut || p.twin) attn_join_kernel<T><<<(unsigned)((p.units * p.unit_rows + 3) / 4), 128, 0, st>>>(g, p.grid);
+  if (p.cut || p.twin) attn_join_kernel<T><<<(unsigned)(p.units * (p.unit_rows / 32)), AT_JOIN, 0, st>>>(g, p.grid);
   return launched("scb_attention");
 }
 
