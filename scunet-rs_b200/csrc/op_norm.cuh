@@ -7,11 +7,20 @@
 //   db_c = sum gz,  dw_c = sum gz xh  (over n and L),
 //   dx = rstd (h - E_g[h] - xh E_g[h xh]).
 //
-// Three launches: per-channel partials of row ranges, their join per group, and the
-// elementwise pass. Statistics are fp32: a thread sums x - K and (x - K)^2 with K its
-// first value of the channel, so that the sum of squares loses nothing to a large mean
-// (K is one of the values, so a K far from the rest is itself part of the spread it
-// stands against), and (count, mean, M2) triples are joined pairwise,
+// Two forms, each with its gradient:
+//  * norm_small_kernel: a picture's rows of a few whole groups fit in one block's shared
+//    memory; the values are read once, one launch.
+//  * norm_stats_kernel, then norm_apply_kernel (norm_grad_sums_kernel, then
+//    norm_grad_apply_kernel): blocks take row ranges of all pictures and leave one partial
+//    per group; the second launch starts while the first one ends, every block joins its
+//    picture's partials itself, and walks its rows backwards, so that what the first pass
+//    read last is still in L2.
+// A thread keeps its channels (a vector of up to 16 bytes) and steps over rows.
+//
+// Statistics are fp32: a thread sums x - K and (x - K)^2 with K its first value of the
+// channel, so that the sum of squares loses nothing to a large mean (K is one of the
+// values, so a K far from the rest is itself part of the spread it stands against), and
+// (count, mean, M2) triples are joined pairwise,
 //   M2 = M2a + M2b + (mb - ma)^2 na nb / (na + nb).
 // No atomics: the order of every sum is fixed by the sizes.
 #pragma once
@@ -21,9 +30,12 @@ namespace scb {
 
 struct NormGeom {
   long n, l;          // pictures, rows of each
+  long first;         // first picture of the launch
   int c, groups, cpg; // channels, groups, channels per group
   int cols;           // vectors of a row
-  int tc, rp;         // vectors of a row that one block takes, rows it takes at once
+  int tc, rp;         // vectors of a row that one block takes (a chunk), rows it takes at once
+  int chunks, slots;  // chunks of a row; groups + chunks - 1 partials of a split: a chunk's
+                      // part of a group is slot group + chunk (a group may span chunks)
   int splits;         // row ranges of a picture
   long x_sn, x_sl;    // element strides of pictures and rows
   long y_sn, y_sl;
@@ -32,21 +44,8 @@ struct NormGeom {
   int act;            // read by the kernels compiled for ACT_ANY
 };
 
-constexpr int NORM_THREADS = 256;
-
-// The narrow vectors take the activation at run time (ACT_ANY).
-template <int ACT>
-__device__ __forceinline__ float act_of(const NormGeom& g, float z) {
-  if (ACT != ACT_ANY) return act_fwd<ACT>(z);
-  return g.act == ACT_RELU ? act_fwd<ACT_RELU>(z) : g.act == ACT_SILU ? act_fwd<ACT_SILU>(z)
-         : g.act == ACT_GELU ? act_fwd<ACT_GELU>(z) : z;
-}
-template <int ACT>
-__device__ __forceinline__ float slope_of(const NormGeom& g, float z) {
-  if (ACT != ACT_ANY) return act_slope<ACT>(z);
-  return g.act == ACT_RELU ? act_slope<ACT_RELU>(z) : g.act == ACT_SILU ? act_slope<ACT_SILU>(z)
-         : g.act == ACT_GELU ? act_slope<ACT_GELU>(z) : 1.f;
-}
+constexpr int NORM_THREADS = 512;  // two blocks an SM: every block reads its picture's partials
+constexpr int NORM_SMALL_BYTES = 184 * 1024;  // shared memory for the small form's values
 
 struct Moments {
   float n, mean, m2;
@@ -57,6 +56,210 @@ __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
   const float d = b.mean - a.mean, f = b.n / n;
   return {n, a.mean + d * f, a.m2 + b.m2 + d * d * a.n * f};
 }
+__device__ __forceinline__ Moments shfl_xor(const Moments& m, int d) {
+  return {__shfl_xor_sync(0xffffffffu, m.n, d), __shfl_xor_sync(0xffffffffu, m.mean, d),
+          __shfl_xor_sync(0xffffffffu, m.m2, d)};
+}
+__device__ __forceinline__ float2 shfl_xor(const float2& v, int d) {
+  return make_float2(__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d));
+}
+__device__ __forceinline__ float2 join(const float2& a, const float2& b) { return make_float2(a.x + b.x, a.y + b.y); }
+// The join over a warp, the same in every lane (operands ordered by lane).
+template <typename S>
+__device__ __forceinline__ S warp_join(S v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const S o = shfl_xor(v, d);
+    v = lane & d ? join(o, v) : join(v, o);
+  }
+  return v;
+}
+
+// V values in fp32 and back.
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& a, float* v) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = to_f32(a.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> repack(const float* v) {
+  Pack<T, V> a;
+#pragma unroll
+  for (int i = 0; i < V; ++i) a.v[i] = from_f32<T>(v[i]);
+  return a;
+}
+
+// Activations of V values. SiLU takes one reciprocal for two values (1/a = b / (ab)): the
+// special function unit, at two operations a value, would bound the pass; e^-z is capped at
+// 2^60, where the product stays finite and z sigmoid(z) is 0 to 1e-17.
+template <int ACT, int V>
+__device__ __forceinline__ void sigmoids(const float* z, float* s) {
+#pragma unroll
+  for (int i = 0; i < V; i += 2) {
+    const float a = 1.f + ex2_approx(fminf(z[i] * -1.4426950408889634f, 60.f));
+    if (i + 1 < V) {
+      const float b = 1.f + ex2_approx(fminf(z[i + 1] * -1.4426950408889634f, 60.f));
+      const float r = rcp_approx(a * b);
+      s[i] = b * r;
+      s[i + 1] = a * r;
+    } else {
+      s[i] = rcp_approx(a);
+    }
+  }
+}
+template <int ACT, int V>
+__device__ __forceinline__ void act_all(const NormGeom& g, float* z) {
+  if (ACT == ACT_SILU) {
+    float s[V];
+    sigmoids<ACT, V>(z, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] *= s[i];
+  } else if (ACT == ACT_ANY) {
+    if (g.act == ACT_SILU) return act_all<ACT_SILU, V>(g, z);
+    if (g.act == ACT_GELU) return act_all<ACT_GELU, V>(g, z);
+    if (g.act == ACT_RELU) return act_all<ACT_RELU, V>(g, z);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = act_fwd<ACT>(z[i]);
+  }
+}
+// z -> act'(z)
+template <int ACT, int V>
+__device__ __forceinline__ void slope_all(const NormGeom& g, float* z) {
+  if (ACT == ACT_SILU) {
+    float s[V];
+    sigmoids<ACT, V>(z, s);
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = s[i] * (1.f + z[i] * (1.f - s[i]));
+  } else if (ACT == ACT_ANY) {
+    if (g.act == ACT_SILU) return slope_all<ACT_SILU, V>(g, z);
+    if (g.act == ACT_GELU) return slope_all<ACT_GELU, V>(g, z);
+    if (g.act == ACT_RELU) return slope_all<ACT_RELU, V>(g, z);
+    return slope_all<ACT_NONE, V>(g, z);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = act_slope<ACT>(z[i]);
+  }
+}
+
+// What a thread needs of its channels: z = x sc + sh (one rounding; sh holds b - mean sc,
+// whose rounding is that of the mean itself).
+template <int V>
+struct Channels {
+  float sc[V], sh[V];
+  __device__ __forceinline__ void load(const NormGeom& g, const float2* stats, int first_group, int c0,
+                                       const float* weight, const float* bias) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = c0 + i;
+      const float2 st = stats[c / g.cpg - first_group];
+      sc[i] = st.y * (weight ? weight[c] : 1.f);
+      sh[i] = fmaf(-st.x, sc[i], bias ? bias[c] : 0.f);
+    }
+  }
+  __device__ __forceinline__ void z(const float* x, float* out) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = fmaf(x[i], sc[i], sh[i]);
+  }
+};
+// xh = x rs + mr of the same channels, for the gradient.
+template <int V>
+struct Hats {
+  float rs[V], mr[V];
+  __device__ __forceinline__ void load(const NormGeom& g, const float2* stats, int first_group, int c0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 st = stats[(c0 + i) / g.cpg - first_group];
+      rs[i] = st.y;
+      mr[i] = -st.x * st.y;
+    }
+  }
+  __device__ __forceinline__ float at(int i, float x) const { return fmaf(x, rs[i], mr[i]); }
+};
+
+// The running sums of a thread, joined over the block's row lanes in shared memory.
+template <int V>
+struct RowMoments {
+  float k[V], s[V], q[V], cnt;
+  __device__ __forceinline__ void clear() {
+    cnt = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) k[i] = s[i] = q[i] = 0.f;
+  }
+  __device__ __forceinline__ void start(const float* v) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) k[i] = v[i];
+  }
+  __device__ __forceinline__ void add(const float* v) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float d = v[i] - k[i];
+      s[i] += d;
+      q[i] += d * d;
+    }
+  }
+  static constexpr int kFloats = 2 * V + 1;  // per thread
+};
+
+// Joins the row lanes' moments per channel into lane 0's places: mean at mem[i * T + t],
+// M2 at mem[(V + i) * T + t] for channel t V + i of the chunk.
+template <int V, int T>
+__device__ __forceinline__ void join_lanes(const RowMoments<V>& r, float* mem, int tc, int rp, int lane) {
+  const int tid = threadIdx.x;
+  float *sm = mem, *sq = mem + V * T, *sn = mem + 2 * V * T;
+  const float inv = r.cnt > 0.f ? 1.f / r.cnt : 0.f;
+  sn[tid] = r.cnt;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    sm[i * T + tid] = r.k[i] + r.s[i] * inv;
+    sq[i * T + tid] = r.cnt > 0.f ? fmaxf(r.q[i] - r.s[i] * r.s[i] * inv, 0.f) : 0.f;
+    if (r.q[i] != r.q[i]) sq[i * T + tid] = r.q[i];  // fmaxf would drop a NaN
+  }
+  int top = 1;
+  while (top < rp) top *= 2;
+  for (int h = top / 2; h >= 1; h /= 2) {
+    __syncthreads();
+    if (lane < h && lane + h < rp) {
+      const int o = tid + h * tc;
+      const float na = sn[tid], nb = sn[o];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int a = i * T;
+        const Moments m = join(Moments{na, sm[a + tid], sq[a + tid]}, Moments{nb, sm[a + o], sq[a + o]});
+        sm[a + tid] = m.mean;
+        sq[a + tid] = m.m2;
+      }
+      sn[tid] = na + nb;
+    }
+  }
+  __syncthreads();
+}
+// The same for two plain sums.
+template <int V, int T>
+__device__ __forceinline__ void add_lanes(const float* a, const float* b, float* mem, int tc, int rp, int lane) {
+  const int tid = threadIdx.x;
+  float *ra = mem, *rb = mem + V * T;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    ra[i * T + tid] = a[i];
+    rb[i * T + tid] = b[i];
+  }
+  int top = 1;
+  while (top < rp) top *= 2;
+  for (int h = top / 2; h >= 1; h /= 2) {
+    __syncthreads();
+    if (lane < h && lane + h < rp) {
+      const int o = tid + h * tc;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        ra[i * T + tid] += ra[i * T + o];
+        rb[i * T + tid] += rb[i * T + o];
+      }
+    }
+  }
+  __syncthreads();
+}
 
 // The row range of split s.
 __device__ __forceinline__ void norm_rows(const NormGeom& g, int s, long& r0, long& r1) {
@@ -64,295 +267,426 @@ __device__ __forceinline__ void norm_rows(const NormGeom& g, int s, long& r0, lo
   r1 = g.l * (s + 1) / g.splits;
 }
 
-// Per (picture, split, channel): mean and M2 of the split's rows -> part[n][split][c].
+// A block's place: picture, split, chunk, its thread's vector and row lane.
+struct NormPlace {
+  long pic, r0, r1;
+  int split, chunk, col, lane;
+  bool on;
+  int c0, c1;  // the chunk's channels
+  __device__ __forceinline__ NormPlace(const NormGeom& g, int vec) {
+    pic = g.first + blockIdx.x / g.splits;
+    split = (int)(blockIdx.x % g.splits);
+    chunk = blockIdx.y;
+    col = chunk * g.tc + threadIdx.x % g.tc;
+    lane = threadIdx.x / g.tc;
+    on = lane < g.rp && col < g.cols;
+    norm_rows(g, split, r0, r1);
+    c0 = chunk * g.tc * vec;
+    c1 = min(c0 + g.tc * vec, g.c);
+  }
+};
+
+// Launch order of the two passes (programmatic dependent launch): the first lets the second
+// start early, the second waits for the first's results before it reads or writes anything.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// First pass: per (picture, split, chunk's part of a group) mean and M2.
 template <typename T, int V>
-__global__ void __launch_bounds__(NORM_THREADS) norm_stats_kernel(const T* __restrict__ x, float2* __restrict__ part,
-                                                                  const NormGeom g) {
+__global__ void __launch_bounds__(NORM_THREADS, 2)
+norm_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, const __grid_constant__ NormGeom g) {
   extern __shared__ float norm_sm[];
-  const int tid = threadIdx.x, col = blockIdx.y * g.tc + tid % g.tc, lane = tid / g.tc;
-  const bool on = lane < g.rp && col < g.cols;
-  long r0, r1;
-  const long pic = blockIdx.x / g.splits;
-  const int split = (int)(blockIdx.x % g.splits);
-  norm_rows(g, split, r0, r1);
-  float k[V], s[V], q[V];
-  float cnt = 0.f;
-#pragma unroll
-  for (int i = 0; i < V; ++i) k[i] = s[i] = q[i] = 0.f;
-  if (on) {
-    const T* p = x + pic * g.x_sn + (long)col * V;
-    long r = r0 + lane;
-    if (r < r1) {
-      Pack<T, V> a;
-      a.load(p + r * g.x_sl);
-#pragma unroll
-      for (int i = 0; i < V; ++i) k[i] = to_f32(a.v[i]);
-      cnt = (float)((r1 - r + g.rp - 1) / g.rp);
-    }
+  let_next_start();
+  const NormPlace p(g, V);
+  RowMoments<V> r;
+  r.clear();
+  long row = p.r0 + p.lane;
+  if (p.on && row < p.r1) {
+    const T* src = x + p.pic * g.x_sn + (long)p.col * V;
+    Pack<T, V> a;
+    float v[V];
+    a.load(src + row * g.x_sl);
+    unpack(a, v);
+    r.start(v);
+    r.cnt = (float)((p.r1 - row + g.rp - 1) / g.rp);
 #pragma unroll 4
-    for (; r < r1; r += g.rp) {
-      Pack<T, V> a;
-      a.load(p + r * g.x_sl);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = to_f32(a.v[i]) - k[i];
-        s[i] += d;
-        q[i] += d * d;
-      }
+    for (; row < p.r1; row += g.rp) {
+      a.load(src + row * g.x_sl);
+      unpack(a, v);
+      r.add(v);
     }
   }
-  // join the block's row lanes, channel by channel, as a tree over lanes
-  float* sn = norm_sm;                    // [256]
-  float* sm = norm_sm + NORM_THREADS;     // [V][256]
-  float* sq = sm + V * NORM_THREADS;      // [V][256]
-  const float inv = cnt > 0.f ? 1.f / cnt : 0.f;
-  sn[tid] = cnt;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    sm[i * NORM_THREADS + tid] = k[i] + s[i] * inv;
-    sq[i * NORM_THREADS + tid] = fmaxf(q[i] - s[i] * s[i] * inv, 0.f);
-  }
-  int top = 1;
-  while (top < g.rp) top *= 2;
-  for (int h = top / 2; h >= 1; h /= 2) {
-    __syncthreads();
-    if (lane < h && lane + h < g.rp) {
-      const int o = tid + h * g.tc;
-      const float na = sn[tid], nb = sn[o];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int a = i * NORM_THREADS;
-        const Moments m = join({na, sm[a + tid], sq[a + tid]}, {nb, sm[a + o], sq[a + o]});
-        sm[a + tid] = m.mean;
-        sq[a + tid] = m.m2;
-      }
-      sn[tid] = na + nb;
+  join_lanes<V, NORM_THREADS>(r, norm_sm, g.tc, g.rp, p.lane);
+  const float rows = (float)(p.r1 - p.r0);
+  float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
+  for (int grp = p.c0 / g.cpg + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
+    Moments m{0.f, 0.f, 0.f};
+    for (int c = max(grp * g.cpg, p.c0) + (threadIdx.x & 31); c < min((grp + 1) * g.cpg, p.c1); c += 32) {
+      const int e = c - p.c0, at = (e % V) * NORM_THREADS + e / V;
+      m = join(m, Moments{rows, norm_sm[at], norm_sm[V * NORM_THREADS + at]});
     }
-  }
-  if (lane == 0 && on) {
-    float2* o = part + (long)blockIdx.x * g.c + (long)col * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = make_float2(sm[i * NORM_THREADS + tid], sq[i * NORM_THREADS + tid]);
+    m = warp_join(m);
+    if ((threadIdx.x & 31) == 0) out[grp] = make_float2(m.mean, m.m2);
   }
 }
 
-__device__ __forceinline__ Moments shfl_down(const Moments& m, int d) {
-  return {__shfl_down_sync(0xffffffffu, m.n, d), __shfl_down_sync(0xffffffffu, m.mean, d),
-          __shfl_down_sync(0xffffffffu, m.m2, d)};
-}
-
-// One block per (group, picture): joins the partials of all splits and channels.
-__global__ void __launch_bounds__(NORM_THREADS) norm_join_kernel(const float2* __restrict__ part,
-                                                                 float* __restrict__ mean, float* __restrict__ rstd,
-                                                                 const NormGeom g) {
-  __shared__ Moments sw[NORM_THREADS / 32];
+// A picture's group, joined over splits (and chunks) by one warp: (mean, rstd).
+__device__ __forceinline__ float2 norm_join(const NormGeom& g, const float2* part, long pic, int grp, int vec) {
+  const int per = g.tc * vec;  // channels of a chunk
+  const int k0 = grp * g.cpg / per, k1 = ((grp + 1) * g.cpg - 1) / per;
   Moments m{0.f, 0.f, 0.f};
-  const long pic = blockIdx.x / g.groups, grp = blockIdx.x % g.groups;
-  for (int i = threadIdx.x; i < g.splits * g.cpg; i += NORM_THREADS) {
-    const int s = i / g.cpg, c = i - s * g.cpg;
+  for (int s = threadIdx.x & 31; s < g.splits; s += 32) {
     long r0, r1;
     norm_rows(g, s, r0, r1);
-    const float2 v = part[(pic * g.splits + s) * g.c + grp * g.cpg + c];
-    m = join(m, {(float)(r1 - r0), v.x, v.y});
+    for (int k = k0; k <= k1; ++k) {
+      const int width = min((grp + 1) * g.cpg, (k + 1) * per) - max(grp * g.cpg, k * per);
+      const float2 v = __ldcg(part + (pic * g.splits + s) * g.slots + grp + k);
+      m = join(m, Moments{(float)(r1 - r0) * (float)width, v.x, v.y});
+    }
   }
-  for (int d = 16; d >= 1; d /= 2) m = join(m, shfl_down(m, d));
-  if ((threadIdx.x & 31) == 0) sw[threadIdx.x >> 5] = m;
+  m = warp_join(m);
+  return make_float2(m.mean, 1.f / sqrtf((m.n > 0.f ? m.m2 / m.n : 0.f) + g.eps));
+}
+
+// Second pass: y = act((x - mean) rstd w + b).
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(NORM_THREADS, 2)
+norm_apply_kernel(const T* x, T* y, const float2* __restrict__ part,
+                  float* __restrict__ mean, float* __restrict__ rstd, const float* __restrict__ weight,
+                  const float* __restrict__ bias, const __grid_constant__ NormGeom g) {
+  extern __shared__ float2 norm_stat[];  // of the chunk's groups
+  const NormPlace p(g, V);
+  const int g0 = p.c0 / g.cpg;
+  wait_for_previous();
+  for (int grp = g0 + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
+    const float2 s = norm_join(g, part, p.pic, grp, V);
+    if ((threadIdx.x & 31) == 0) {
+      norm_stat[grp - g0] = s;
+      if (p.split == 0 && grp * g.cpg >= p.c0) {  // the chunk that holds the group's start
+        if (mean) mean[p.pic * g.groups + grp] = s.x;
+        if (rstd) rstd[p.pic * g.groups + grp] = s.y;
+      }
+    }
+  }
   __syncthreads();
-  if (threadIdx.x < 32) {
-    m = threadIdx.x < NORM_THREADS / 32 ? sw[threadIdx.x] : Moments{0.f, 0.f, 0.f};
-    for (int d = NORM_THREADS / 64; d >= 1; d /= 2) m = join(m, shfl_down(m, d));
-    if (threadIdx.x == 0) {
-      mean[pic * g.groups + grp] = m.mean;
-      rstd[pic * g.groups + grp] = 1.f / sqrtf((m.n > 0.f ? m.m2 / m.n : 0.f) + g.eps);
+  if (!p.on || p.r0 + p.lane >= p.r1) return;
+  Channels<V> ch;
+  ch.load(g, norm_stat, g0, p.col * V, weight, bias);
+  const T* src = x + p.pic * g.x_sn + (long)p.col * V;
+  T* dst = y + p.pic * g.y_sn + (long)p.col * V;
+  // batches of loads before their stores: y may be x, so the compiler must not reorder them
+  constexpr int kBatch = sizeof(Pack<T, V>) == 16 ? 2 : 4;
+  const long steps = (p.r1 - p.r0 - p.lane - 1) / g.rp;
+  for (long row = p.r0 + p.lane + steps * g.rp; row >= p.r0; row -= kBatch * g.rp) {
+    Pack<T, V> a[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (row - b * g.rp >= p.r0) a[b].load(src + (row - b * g.rp) * g.x_sl);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (row - b * g.rp < p.r0) break;
+      float v[V];
+      unpack(a[b], v);
+      ch.z(v, v);
+      act_all<ACT, V>(g, v);
+      repack<T, V>(v).store(dst + (row - b * g.rp) * g.y_sl);
     }
   }
 }
 
-// y = act(x scale_c + shift_c), the pass over the values.
+// gz = dy act'(z) of V values.
+template <int ACT, int V>
+__device__ __forceinline__ void grad_z(const NormGeom& g, const Channels<V>& ch, const float* x, const float* dy,
+                                       float* gz) {
+  ch.z(x, gz);
+  slope_all<ACT, V>(g, gz);
+#pragma unroll
+  for (int i = 0; i < V; ++i) gz[i] *= dy[i];
+}
+
+// (mean, rstd) of the chunk's groups into shared memory.
+__device__ __forceinline__ void grad_stats(const NormGeom& g, float2* stats, int g0, int c1, const float* mean,
+                                           const float* rstd, long pic) {
+  for (int grp = g0 + threadIdx.x; grp * g.cpg < c1; grp += blockDim.x)
+    stats[grp - g0] = make_float2(mean[pic * g.groups + grp], rstd[pic * g.groups + grp]);
+}
+
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS)
-norm_apply_kernel(const T* __restrict__ x, T* __restrict__ y, const float* __restrict__ mean,
-                  const float* __restrict__ rstd, const float* __restrict__ weight, const float* __restrict__ bias,
-                  const NormGeom g) {
-  const int tid = threadIdx.x, col = blockIdx.y * g.tc + tid % g.tc, lane = tid / g.tc;
-  if (lane >= g.rp || col >= g.cols) return;
-  const long pic = blockIdx.x / g.splits;
-  const int split = (int)(blockIdx.x % g.splits);
-  float mu[V], sc[V], sh[V];
+__device__ __forceinline__ void add_grad(const NormGeom& g, const Channels<V>& ch, const Hats<V>& hat,
+                                         const Pack<T, V>& a, const Pack<T, V>& e, float* sa, float* sb) {
+  float v[V], d[V], gz[V];
+  unpack(a, v);
+  unpack(e, d);
+  grad_z<ACT, V>(g, ch, v, d, gz);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = col * V + i;
-    const long k = pic * g.groups + c / g.cpg;
-    mu[i] = mean[k];
-    sc[i] = rstd[k] * (weight ? weight[c] : 1.f);
-    sh[i] = bias ? bias[c] : 0.f;
-  }
-  long r0, r1;
-  norm_rows(g, split, r0, r1);
-  const T* p = x + pic * g.x_sn + (long)col * V;
-  T* o = y + pic * g.y_sn + (long)col * V;
-#pragma unroll 4
-  for (long r = r0 + lane; r < r1; r += g.rp) {
-    Pack<T, V> a;
-    a.load(p + r * g.x_sl);
-#pragma unroll
-    for (int i = 0; i < V; ++i) a.v[i] = from_f32<T>(act_of<ACT>(g, (to_f32(a.v[i]) - mu[i]) * sc[i] + sh[i]));
-    a.store(o + r * g.y_sl);
+    sa[i] += gz[i];
+    sb[i] = fmaf(gz[i], hat.at(i, v[i]), sb[i]);
   }
 }
 
-// Per (picture, split, channel): sums of gz and gz xh over the split's rows.
+// First pass of the gradient: per (picture, split) the channels' sums of gz and gz xh for dw
+// and db, and the parts of the groups' sums of h and h xh.
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS)
+__global__ void __launch_bounds__(NORM_THREADS, 2)
 norm_grad_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean,
                       const float* __restrict__ rstd, const float* __restrict__ weight,
-                      const float* __restrict__ bias, float2* __restrict__ part, const NormGeom g) {
-  extern __shared__ float norm_sm[];
-  const int tid = threadIdx.x, col = blockIdx.y * g.tc + tid % g.tc, lane = tid / g.tc;
-  const bool on = lane < g.rp && col < g.cols;
-  const long pic = blockIdx.x / g.splits;
-  const int split = (int)(blockIdx.x % g.splits);
+                      const float* __restrict__ bias, float2* __restrict__ part, float2* __restrict__ cpart,
+                      const __grid_constant__ NormGeom g) {
+  extern __shared__ float norm_sm[];  // [2][V][threads], then the chunk's groups' statistics
+  let_next_start();
+  const NormPlace p(g, V);
+  const int g0 = p.c0 / g.cpg;
+  float2* stats = reinterpret_cast<float2*>(norm_sm + 2 * V * NORM_THREADS);
+  grad_stats(g, stats, g0, p.c1, mean, rstd, p.pic);
+  __syncthreads();
   float sa[V], sb[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.f;
-  if (on) {
-    float mu[V], rs[V], w[V], b[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = col * V + i;
-      const long k = pic * g.groups + c / g.cpg;
-      mu[i] = mean[k];
-      rs[i] = rstd[k];
-      w[i] = weight ? weight[c] : 1.f;
-      b[i] = bias ? bias[c] : 0.f;
-    }
-    long r0, r1;
-    norm_rows(g, split, r0, r1);
-    const T* p = x + pic * g.x_sn + (long)col * V;
-    const T* d = dy + pic * g.d_sn + (long)col * V;
-#pragma unroll 2
-    for (long r = r0 + lane; r < r1; r += g.rp) {
+  if (p.on) {
+    Channels<V> ch;
+    Hats<V> hat;
+    ch.load(g, stats, g0, p.col * V, weight, bias);
+    hat.load(g, stats, g0, p.col * V);
+    const T* src = x + p.pic * g.x_sn + (long)p.col * V;
+    const T* del = dy + p.pic * g.d_sn + (long)p.col * V;
+#pragma unroll 4
+    for (long row = p.r0 + p.lane; row < p.r1; row += g.rp) {
       Pack<T, V> a, e;
-      a.load(p + r * g.x_sl);
-      e.load(d + r * g.d_sl);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xh = (to_f32(a.v[i]) - mu[i]) * rs[i];
-        const float gz = to_f32(e.v[i]) * slope_of<ACT>(g, xh * w[i] + b[i]);
-        sa[i] += gz;
-        sb[i] += gz * xh;
-      }
+      a.load(src + row * g.x_sl);
+      e.load(del + row * g.d_sl);
+      add_grad<T, V, ACT>(g, ch, hat, a, e, sa, sb);
     }
   }
-  float* ra = norm_sm;                     // [V][256]
-  float* rb = norm_sm + V * NORM_THREADS;  // [V][256]
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    ra[i * NORM_THREADS + tid] = sa[i];
-    rb[i * NORM_THREADS + tid] = sb[i];
-  }
-  int top = 1;
-  while (top < g.rp) top *= 2;
-  for (int h = top / 2; h >= 1; h /= 2) {
-    __syncthreads();
-    if (lane < h && lane + h < g.rp) {
-      const int o = tid + h * g.tc;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        ra[i * NORM_THREADS + tid] += ra[i * NORM_THREADS + o];
-        rb[i * NORM_THREADS + tid] += rb[i * NORM_THREADS + o];
-      }
+  add_lanes<V, NORM_THREADS>(sa, sb, norm_sm, g.tc, g.rp, p.lane);
+  float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
+  float2* cout = cpart + (p.pic * g.splits + p.split) * g.c;
+  for (int grp = g0 + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
+    float2 m = make_float2(0.f, 0.f);
+    for (int c = max(grp * g.cpg, p.c0) + (threadIdx.x & 31); c < min((grp + 1) * g.cpg, p.c1); c += 32) {
+      const int e = c - p.c0, at = (e % V) * NORM_THREADS + e / V;
+      const float2 s = make_float2(norm_sm[at], norm_sm[V * NORM_THREADS + at]);
+      cout[c] = s;
+      const float w = weight ? weight[c] : 1.f;
+      m = join(m, make_float2(w * s.x, w * s.y));
     }
-  }
-  if (lane == 0 && on) {
-    float2* o = part + (long)blockIdx.x * g.c + (long)col * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = make_float2(ra[i * NORM_THREADS + tid], rb[i * NORM_THREADS + tid]);
+    m = warp_join(m);
+    if ((threadIdx.x & 31) == 0) out[grp] = m;
   }
 }
 
-// One block per channel: joins the splits. sums[n][c] = the picture's (sum gz, sum gz xh);
-// dw and db add the pictures.
-__global__ void __launch_bounds__(32) norm_grad_join_kernel(const float2* __restrict__ part, float2* __restrict__ sums,
-                                                            float* __restrict__ dweight, float* __restrict__ dbias,
-                                                            const NormGeom g) {
-  const int c = blockIdx.x;
-  float ta = 0.f, tb = 0.f;
-  for (long pic = 0; pic < g.n; ++pic) {
-    float a = 0.f, b = 0.f;
-    for (int s = threadIdx.x; s < g.splits; s += 32) {
-      const float2 v = part[(pic * g.splits + s) * g.c + c];
-      a += v.x;
-      b += v.y;
+// (E[h], E[h xh]) of a picture's group, joined by one warp.
+__device__ __forceinline__ float2 norm_grad_join(const NormGeom& g, const float2* part, long pic, int grp, int vec) {
+  const int per = g.tc * vec, k0 = grp * g.cpg / per, k1 = ((grp + 1) * g.cpg - 1) / per;
+  float2 m = make_float2(0.f, 0.f);
+  for (int s = threadIdx.x & 31; s < g.splits; s += 32)
+    for (int k = k0; k <= k1; ++k) m = join(m, __ldcg(part + (pic * g.splits + s) * g.slots + grp + k));
+  m = warp_join(m);
+  const float inv = 1.f / ((float)g.l * (float)g.cpg);
+  return make_float2(m.x * inv, m.y * inv);
+}
+
+// dx = gz sc - rs E[h] - xh rs E[h xh] of one vector (sc = rs w).
+template <int V>
+struct GradMeans {
+  float m1[V], m2[V];  // rs E[h], rs E[h xh]
+  __device__ __forceinline__ void load(const NormGeom& g, const Hats<V>& hat, const float2* means, int first_group,
+                                       int c0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 m = means[(c0 + i) / g.cpg - first_group];
+      m1[i] = hat.rs[i] * m.x;
+      m2[i] = hat.rs[i] * m.y;
     }
-    for (int d = 16; d >= 1; d /= 2) {
-      a += __shfl_down_sync(0xffffffffu, a, d);
-      b += __shfl_down_sync(0xffffffffu, b, d);
-    }
-    if (threadIdx.x == 0) sums[pic * g.c + c] = make_float2(a, b);
-    ta += a;
-    tb += b;
   }
-  if (threadIdx.x == 0) {
-    if (dbias) dbias[c] = ta;
-    if (dweight) dweight[c] = tb;
-  }
+};
+template <typename T, int V, int ACT>
+__device__ __forceinline__ Pack<T, V> grad_x(const NormGeom& g, const Channels<V>& ch, const Hats<V>& hat,
+                                             const GradMeans<V>& m, const Pack<T, V>& a, const Pack<T, V>& e) {
+  float v[V], d[V], gz[V];
+  unpack(a, v);
+  unpack(e, d);
+  grad_z<ACT, V>(g, ch, v, d, gz);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = fmaf(gz[i], ch.sc[i], -m.m1[i]) - hat.at(i, v[i]) * m.m2[i];
+  return repack<T, V>(v);
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS)
-norm_grad_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, T* __restrict__ dx,
+__global__ void __launch_bounds__(NORM_THREADS, 2)
+norm_grad_apply_kernel(const T* dy, const T* x, T* dx,
                        const float* __restrict__ mean, const float* __restrict__ rstd,
                        const float* __restrict__ weight, const float* __restrict__ bias,
-                       const float2* __restrict__ sums, const NormGeom g) {
-  const int tid = threadIdx.x, col = blockIdx.y * g.tc + tid % g.tc, lane = tid / g.tc;
-  if (lane >= g.rp || col >= g.cols) return;
-  const long pic = blockIdx.x / g.splits;
-  const int split = (int)(blockIdx.x % g.splits);
-  float mu[V], rs[V], w[V], b[V], m1[V], m2[V];
-  int last = -1;
+                       const float2* __restrict__ part, const __grid_constant__ NormGeom g) {
+  extern __shared__ float2 norm_stat[];  // (mean, rstd), then (E[h], E[h xh]) of the chunk's groups
+  const NormPlace p(g, V);
+  const int g0 = p.c0 / g.cpg, ng = (p.c1 - 1) / g.cpg - g0 + 1;
+  grad_stats(g, norm_stat, g0, p.c1, mean, rstd, p.pic);
+  wait_for_previous();
+  for (int grp = g0 + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
+    const float2 m = norm_grad_join(g, part, p.pic, grp, V);
+    if ((threadIdx.x & 31) == 0) norm_stat[ng + grp - g0] = m;
+  }
+  __syncthreads();
+  if (!p.on || p.r0 + p.lane >= p.r1) return;
+  Channels<V> ch;
+  ch.load(g, norm_stat, g0, p.col * V, weight, bias);
+  Hats<V> hat;
+  GradMeans<V> m;
+  hat.load(g, norm_stat, g0, p.col * V);
+  m.load(g, hat, norm_stat + ng, g0, p.col * V);
+  const T* src = x + p.pic * g.x_sn + (long)p.col * V;
+  const T* del = dy + p.pic * g.d_sn + (long)p.col * V;
+  T* dst = dx + p.pic * g.y_sn + (long)p.col * V;
+  const long steps = (p.r1 - p.r0 - p.lane - 1) / g.rp;
+  constexpr int kBatch = 2;
+  for (long row = p.r0 + p.lane + steps * g.rp; row >= p.r0; row -= kBatch * g.rp) {
+    Pack<T, V> a[kBatch], e[kBatch];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int c = col * V + i, grp = c / g.cpg;
-    const long k = pic * g.groups + grp;
-    mu[i] = mean[k];
-    rs[i] = rstd[k];
-    w[i] = weight ? weight[c] : 1.f;
-    b[i] = bias ? bias[c] : 0.f;
-    if (i > 0 && grp == last) {
-      m1[i] = m1[i - 1];
-      m2[i] = m2[i - 1];
-    } else {
-      float a1 = 0.f, a2 = 0.f;
-      for (int j = 0; j < g.cpg; ++j) {
-        const float2 v = sums[pic * g.c + grp * g.cpg + j];
-        const float wj = weight ? weight[grp * g.cpg + j] : 1.f;
-        a1 += wj * v.x;
-        a2 += wj * v.y;
+    for (int k = 0; k < kBatch; ++k)
+      if (row - k * g.rp >= p.r0) {
+        a[k].load(src + (row - k * g.rp) * g.x_sl);
+        e[k].load(del + (row - k * g.rp) * g.d_sl);
       }
-      const float inv = 1.f / ((float)g.l * (float)g.cpg);
-      m1[i] = a1 * inv;
-      m2[i] = a2 * inv;
-      last = grp;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (row - k * g.rp >= p.r0)
+        grad_x<T, V, ACT>(g, ch, hat, m, a[k], e[k]).store(dst + (row - k * g.rp) * g.y_sl);
+  }
+}
+
+// dw and db: one warp a channel joins `parts` partials (pictures x splits).
+__global__ void __launch_bounds__(256) norm_grad_params_kernel(const float2* __restrict__ cpart, long parts,
+                                                                        int c, float* __restrict__ dweight,
+                                                                        float* __restrict__ dbias) {
+  // 32 neighbouring channels a block, eight threads each
+  __shared__ float2 sums[8][33];
+  const int ch = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
+  float2 m = make_float2(0.f, 0.f);
+  if (ch < c)
+    for (long k = lane; k < parts; k += 8) m = join(m, cpart[k * c + ch]);
+  sums[lane][threadIdx.x & 31] = m;
+  __syncthreads();
+  if (lane == 0 && ch < c) {
+    for (int k = 1; k < 8; ++k) m = join(m, sums[k][threadIdx.x]);
+    if (dbias) dbias[ch] = m.x;
+    if (dweight) dweight[ch] = m.y;
+  }
+}
+
+// The small form: block (picture, chunk of whole groups), the chunk's values in shared
+// memory; kT threads: 128 where the values are few and blocks many, else 512. GRAD: x and dy, dx out; the channels' sums go to dw and db when there is one
+// picture, else to cpart.
+template <typename T, int V, bool GRAD, int kT>
+__global__ void __launch_bounds__(kT)
+norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
+                  float* __restrict__ rstd, const float* __restrict__ weight, const float* __restrict__ bias,
+                  float* __restrict__ dweight, float* __restrict__ dbias, float2* __restrict__ cpart,
+                  const __grid_constant__ NormGeom g) {
+  extern __shared__ __align__(16) float norm_sm[];
+  // [2 V + 1][threads] lanes; (mean, rstd), (E[h], E[h xh]) of the groups; the values
+  float2* stats = reinterpret_cast<float2*>(norm_sm + (2 * V + 1) * kT);
+  const NormPlace p(g, V);
+  const int g0 = p.c0 / g.cpg, ng = (p.c1 - p.c0) / g.cpg;
+  Pack<T, V>* keep = reinterpret_cast<Pack<T, V>*>(norm_sm + (2 * V + 1) * kT + 4 * ((g.tc * V / g.cpg + 3) / 4 * 4));
+  Pack<T, V>* keep_d = keep + (GRAD ? g.l * g.tc : 0);
+  const int t = threadIdx.x % g.tc;
+  const T* src = x + p.pic * g.x_sn + (long)p.col * V;
+  const T* del = GRAD ? dy + p.pic * g.d_sn + (long)p.col * V : nullptr;
+  if (!GRAD) {
+    RowMoments<V> r;
+    r.clear();
+    if (p.on && p.lane < g.l) {
+      Pack<T, V> a;
+      float v[V];
+      a.load(src + p.lane * g.x_sl);
+      unpack(a, v);
+      r.start(v);
+      r.cnt = (float)((g.l - p.lane + g.rp - 1) / g.rp);
+#pragma unroll 4
+      for (long row = p.lane; row < g.l; row += g.rp) {
+        a.load(src + row * g.x_sl);
+        keep[row * g.tc + t] = a;
+        unpack(a, v);
+        r.add(v);
+      }
+    }
+    join_lanes<V, kT>(r, norm_sm, g.tc, g.rp, p.lane);
+    for (int k = threadIdx.x >> 5; k < ng; k += kT / 32) {
+      Moments m{0.f, 0.f, 0.f};
+      for (int e = k * g.cpg + (threadIdx.x & 31); e < (k + 1) * g.cpg; e += 32) {
+        const int at = (e % V) * kT + e / V;
+        m = join(m, Moments{(float)g.l, norm_sm[at], norm_sm[V * kT + at]});
+      }
+      m = warp_join(m);
+      if ((threadIdx.x & 31) == 0) {
+        const float rs = 1.f / sqrtf((m.n > 0.f ? m.m2 / m.n : 0.f) + g.eps);
+        stats[k] = make_float2(m.mean, rs);
+        if (mean) mean[p.pic * g.groups + g0 + k] = m.mean;
+        if (rstd) rstd[p.pic * g.groups + g0 + k] = rs;
+      }
+    }
+  } else {
+    grad_stats(g, stats, g0, p.c1, mean, rstd, p.pic);
+  }
+  __syncthreads();
+  Channels<V> ch;
+  Hats<V> hat;
+  if (p.on) {
+    ch.load(g, stats, g0, p.col * V, weight, bias);
+    if (GRAD) hat.load(g, stats, g0, p.col * V);
+  }
+  T* dst = y + p.pic * g.y_sn + (long)p.col * V;
+  if constexpr (!GRAD) {
+    if (p.on)
+      for (long row = p.lane; row < g.l; row += g.rp) {
+        float v[V];
+        unpack(keep[row * g.tc + t], v);
+        ch.z(v, v);
+        act_all<ACT_ANY, V>(g, v);
+        repack<T, V>(v).store(dst + row * g.y_sl);
+      }
+  } else {
+  float sa[V], sb[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.f;
+  if (p.on) {
+#pragma unroll 2
+    for (long row = p.lane; row < g.l; row += g.rp) {
+      Pack<T, V> a, e;
+      a.load(src + row * g.x_sl);
+      e.load(del + row * g.d_sl);
+      keep[row * g.tc + t] = a;
+      keep_d[row * g.tc + t] = e;
+      add_grad<T, V, ACT_ANY>(g, ch, hat, a, e, sa, sb);
     }
   }
-  long r0, r1;
-  norm_rows(g, split, r0, r1);
-  const T* p = x + pic * g.x_sn + (long)col * V;
-  const T* d = dy + pic * g.d_sn + (long)col * V;
-  T* o = dx + pic * g.y_sn + (long)col * V;
-#pragma unroll 2
-  for (long r = r0 + lane; r < r1; r += g.rp) {
-    Pack<T, V> a, e;
-    a.load(p + r * g.x_sl);
-    e.load(d + r * g.d_sl);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float xh = (to_f32(a.v[i]) - mu[i]) * rs[i];
-      const float h = to_f32(e.v[i]) * slope_of<ACT>(g, xh * w[i] + b[i]) * w[i];
-      a.v[i] = from_f32<T>(rs[i] * (h - m1[i] - xh * m2[i]));
+  add_lanes<V, kT>(sa, sb, norm_sm, g.tc, g.rp, p.lane);
+  float2* means = stats + ng;
+  for (int k = threadIdx.x >> 5; k < ng; k += kT / 32) {
+    float2 m = make_float2(0.f, 0.f);
+    for (int e = k * g.cpg + (threadIdx.x & 31); e < (k + 1) * g.cpg; e += 32) {
+      const int at = (e % V) * kT + e / V, c = p.c0 + e;
+      const float2 s = make_float2(norm_sm[at], norm_sm[V * kT + at]);
+      const float w = weight ? weight[c] : 1.f;
+      m = join(m, make_float2(w * s.x, w * s.y));
+      if (cpart) {
+        cpart[p.pic * g.c + c] = s;
+      } else {
+        if (dbias) dbias[c] = s.x;
+        if (dweight) dweight[c] = s.y;
+      }
     }
-    a.store(o + r * g.y_sl);
+    m = warp_join(m);
+    const float inv = 1.f / ((float)g.l * (float)g.cpg);
+    if ((threadIdx.x & 31) == 0) means[k] = make_float2(m.x * inv, m.y * inv);
+  }
+  __syncthreads();
+  if (!p.on) return;
+  GradMeans<V> m;
+  m.load(g, hat, means, g0, p.col * V);
+  for (long row = p.lane; row < g.l; row += g.rp)
+    grad_x<T, V, ACT_ANY>(g, ch, hat, m, keep[row * g.tc + t], keep_d[row * g.tc + t]).store(dst + row * g.y_sl);
   }
 }
 

@@ -11,7 +11,10 @@
 //                pair j of an axis whose pairs start at f
 //
 // The angles are shared by all heads of q and k: a block takes some tokens, computes their
-// P sines and cosines once into shared memory and then streams the heads through.
+// P cosines and sines once into shared memory, then streams the heads through, neighbouring
+// lanes on neighbouring vectors of a token's heads. An item is V pairs in two vectors of V
+// channels (interleaved: neighbouring ones), or V copied channels past the last pair.
+// Bound by memory: x read once, written once.
 #pragma once
 #include "ops_common.cuh"
 
@@ -21,6 +24,23 @@ constexpr int ROT_AXES = 4;
 constexpr int ROT_THREADS = 256;
 enum : int { ROT_HALF = 0, ROT_INTERLEAVED = 1, ROT_AXIAL = 2 };
 enum : int { POS_I32 = 0, POS_I64 = 1, POS_F32 = 2 };
+
+// n / d for 32-bit n: (n * m) >> 32 >> s with m = ceil(2^(32 + s) / d), s = ceil(log2 d), where
+// m has 33 bits; the top one is added by hand (Granlund and Montgomery, division by
+// invariant integers using multiplication).
+struct Divide {
+  unsigned d, m, s1, s2;
+  __host__ static Divide by(unsigned d) {
+    unsigned l = 0;
+    while (l < 32 && (1ull << l) < d) ++l;
+    const unsigned m = (unsigned)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+    return {d, m, l < 1 ? l : 1, l > 1 ? l - 1 : 0};
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const {
+    const unsigned t = __umulhi(m, n);
+    return (t + ((n - t) >> s1)) >> s2;
+  }
+};
 
 struct RotTensor {
   const void* x;
@@ -40,6 +60,9 @@ struct RotGeom {
   const float* freq;
   float sign;           // -1: the inverse rotation
   int per_block;        // tokens of a block
+  int vecs;             // items of a head
+  unsigned items;       // items of a token: vecs * (heads of q and k)
+  Divide by_items, by_vecs, by_l, by_pairs;
 };
 
 __device__ __forceinline__ float rot_position(const RotGeom& g, long i) {
@@ -48,51 +71,102 @@ __device__ __forceinline__ float rot_position(const RotGeom& g, long i) {
   return static_cast<const float*>(g.pos)[i];
 }
 
-template <typename T, int LAYOUT>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const RotGeom g) {
-  extern __shared__ float2 rot_cs[];  // [tokens of the block][pairs]: cos, sin
+// Where an item's channels lie: V at `lo` and V at `hi` (hi < 0: copied channels only); its
+// first pair is `p`. Interleaved items of V > 1 are 2 V neighbouring channels, of which
+// those past the last pair are left as they are.
+struct RotItem {
+  int lo, hi, p;
+};
+template <int LAYOUT, int V>
+__device__ __forceinline__ RotItem rot_item(const RotGeom& g, int v) {
+  const int p = V * v;
+  if (LAYOUT == ROT_INTERLEAVED && V > 1) return {2 * p, 2 * p + V, p};
+  if (p >= g.pairs) return {p + g.pairs, -1, p};
+  if (LAYOUT == ROT_INTERLEAVED) return {2 * p, 2 * p + 1, p};
+  if (LAYOUT == ROT_HALF) return {p, p + g.pairs, p};
+  int a = 0;
+  while (a + 1 < g.axes && p >= g.first[a + 1]) ++a;
+  return {p + g.first[a], p + g.first[a + 1], p};
+}
+
+template <typename T, int LAYOUT, int V>
+__device__ __forceinline__ void rotate(const RotGeom& g, const float2* cs, const RotItem& it,
+                                       Pack<T, V>& a, Pack<T, V>& b) {
+  if (LAYOUT == ROT_INTERLEAVED && V > 1) {
+    // a and b are the two halves of 2 V neighbouring channels
+    T* e[2] = {a.v, b.v};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      T &x = e[2 * i / V][2 * i % V], &y = e[(2 * i + 1) / V][(2 * i + 1) % V];
+      if (it.p + i < g.pairs) {
+        const float2 c = cs[it.p + i];
+        const float u = to_f32(x), v = to_f32(y);
+        x = from_f32<T>(u * c.x - v * c.y);
+        y = from_f32<T>(u * c.y + v * c.x);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 c = cs[it.p + i];
+      const float u = to_f32(a.v[i]), v = to_f32(b.v[i]);
+      a.v[i] = from_f32<T>(u * c.x - v * c.y);
+      b.v[i] = from_f32<T>(u * c.y + v * c.x);
+    }
+  }
+}
+
+template <typename T, int LAYOUT, int V>
+__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(const __grid_constant__ RotGeom g) {
+  extern __shared__ __align__(16) float2 rot_cs[];  // [tokens of the block][pairs]: cos, sin
   const long t0 = (long)blockIdx.x * g.per_block;
   const int nt = (int)min((long)g.per_block, g.tokens - t0);
-  for (int i = threadIdx.x; i < nt * g.pairs; i += ROT_THREADS) {
-    const int tk = i / g.pairs, p = i - tk * g.pairs;
-    const long tok = t0 + tk, b = tok / g.l, l = tok - b * g.l;
+  const long b0 = t0 / g.l;
+  const unsigned l0 = (unsigned)(t0 - b0 * g.l);  // l0 + per_block < 2^32: l is below 2^31
+  for (unsigned i = threadIdx.x; i < (unsigned)nt * g.pairs; i += ROT_THREADS) {
+    const unsigned tk = g.by_pairs.div(i), p = i - tk * g.pairs;
+    const unsigned over = g.by_l.div(l0 + tk), l = l0 + tk - over * (unsigned)g.l;
     int a = 0;
-    while (a + 1 < g.axes && p >= g.first[a + 1]) ++a;
+    while (a + 1 < g.axes && (int)p >= g.first[a + 1]) ++a;
     float s, c;
-    sincosf(rot_position(g, b * g.pos_sb + l * g.pos_sl + a * g.pos_sa) * g.freq[p], &s, &c);
+    sincosf(rot_position(g, (b0 + over) * g.pos_sb + l * g.pos_sl + a * g.pos_sa) * g.freq[p], &s, &c);
     rot_cs[i] = make_float2(c, s * g.sign);
   }
   __syncthreads();
-  const int rest = g.d - 2 * g.pairs, items = g.pairs + rest;  // one pair or one copied channel each
-  for (int w = 0; w < 2; ++w) {
-    const RotTensor& q = g.t[w];
-    const int per_tok = q.heads * items;
-    for (int i = threadIdx.x; i < nt * per_tok; i += ROT_THREADS) {
-      const int tk = i / per_tok, r = i - tk * per_tok, h = r / items, p = r - h * items;
-      const long tok = t0 + tk, b = tok / g.l, l = tok - b * g.l;
-      const T* x = static_cast<const T*>(q.x) + b * q.x_sb + l * q.x_sl + h * q.x_sh;
-      T* y = static_cast<T*>(q.y) + b * q.y_sb + l * q.y_sl + h * q.y_sh;
-      if (p >= g.pairs) {
-        y[p + g.pairs] = x[p + g.pairs];
-        continue;
+  // two items at a time, both loaded before either is stored: y may be x
+  constexpr int kBatch = 2;
+  const unsigned all = (unsigned)nt * g.items;
+  for (unsigned i0 = threadIdx.x; i0 < all; i0 += kBatch * ROT_THREADS) {
+    Pack<T, V> a[kBatch], b[kBatch];
+    T* y[kBatch];
+    RotItem it[kBatch];
+    unsigned tk[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const unsigned i = i0 + k * ROT_THREADS;
+      if (i >= all) continue;
+      tk[k] = g.by_items.div(i);
+      unsigned r = i - tk[k] * g.items;
+      const unsigned q_items = g.t[0].heads * g.vecs;
+      const int w = r >= q_items;
+      r -= w ? q_items : 0;
+      const unsigned h = g.by_vecs.div(r);
+      it[k] = rot_item<LAYOUT, V>(g, (int)(r - h * g.vecs));
+      const unsigned over = g.by_l.div(l0 + tk[k]), l = l0 + tk[k] - over * (unsigned)g.l;
+      const RotTensor& t = g.t[w];
+      const T* x = static_cast<const T*>(t.x) + (b0 + over) * t.x_sb + l * t.x_sl + h * t.x_sh + it[k].lo;
+      y[k] = static_cast<T*>(t.y) + (b0 + over) * t.y_sb + l * t.y_sl + h * t.y_sh + it[k].lo;
+      a[k].load(x);
+      if (it[k].hi >= 0) b[k].load(x + (it[k].hi - it[k].lo));
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (i0 + k * ROT_THREADS >= all) continue;
+      if (it[k].hi >= 0) {
+        rotate<T, LAYOUT, V>(g, rot_cs + tk[k] * g.pairs, it[k], a[k], b[k]);
+        b[k].store(y[k] + (it[k].hi - it[k].lo));
       }
-      int lo, hi;
-      if (LAYOUT == ROT_HALF) {
-        lo = p;
-        hi = p + g.pairs;
-      } else if (LAYOUT == ROT_INTERLEAVED) {
-        lo = 2 * p;
-        hi = lo + 1;
-      } else {
-        int a = 0;
-        while (a + 1 < g.axes && p >= g.first[a + 1]) ++a;
-        lo = p + g.first[a];
-        hi = lo + g.first[a + 1] - g.first[a];
-      }
-      const float2 cs = rot_cs[tk * g.pairs + p];
-      const float u = to_f32(x[lo]), v = to_f32(x[hi]);
-      y[lo] = from_f32<T>(u * cs.x - v * cs.y);
-      y[hi] = from_f32<T>(u * cs.y + v * cs.x);
+      a[k].store(y[k]);
     }
   }
 }

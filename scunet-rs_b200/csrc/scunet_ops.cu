@@ -53,31 +53,81 @@ int sm_count() {
 // ---------------------------------------------------------------------------- group norm
 const long kMaxBlocks = 0x7fffffffl;
 
-// Vectors per row, block tiling and splits of a group norm. `vec`: elements per access.
-void norm_plan(NormGeom& g, int vec, int sms) {
+// What a group norm's launches look like.
+struct NormPlan {
+  NormGeom g;
+  bool small;
+  int threads;        // of the small form
+  size_t smem;        // of the small form
+  long pictures;      // of each launch of the two-pass form
+  size_t part, cpart; // float2 of the workspace: the groups' partials, the channels'
+};
+
+// `vec` elements per access of `es` bytes. The two-pass form takes its pictures a few at a
+// time where all of them are more than L2 keeps but some are not, so that the second pass
+// finds the first one's reads there.
+NormPlan norm_plan(NormGeom g, int vec, int es, bool grad, int sms) {
+  NormPlan p{};
   g.cpg = g.c / g.groups;
   g.cols = g.c / vec;
+  const int bufs = grad ? 2 : 1;
+  // ---- small: whole groups whose values fit; at least 64 bytes of a row (two sectors), and
+  // some work for a block
+  int unit = g.cpg;
+  while (unit % vec) unit += g.cpg;
+  const auto fits = [&](long cc) {
+    return cc <= 512L * vec && (double)g.l * cc * es * bufs <= NORM_SMALL_BYTES && cc / g.cpg <= 512;
+  };
+  if (fits(unit)) {
+    long cc = unit;
+    while (cc < g.c && fits(cc + unit) && (cc * es < 64 || (double)g.l * cc * es * bufs < 8192)) cc += unit;
+    p.small = true;
+    p.threads = (double)g.l * cc * es * bufs <= 16384 && cc <= 128L * vec ? 128 : 512;
+    g.tc = (int)(cc / vec);
+    g.rp = p.threads / g.tc;
+    g.chunks = (int)((g.c + cc - 1) / cc);
+    g.splits = 1;
+    p.smem = 4 * ((size_t)(2 * vec + 1) * p.threads + 4 * ((cc / g.cpg + 3) / 4 * 4)) + (size_t)g.l * cc * es * bufs;
+    p.cpart = grad && g.n > 1 ? (size_t)g.n * g.c : 0;
+    p.g = g;
+    return p;
+  }
+  // ---- two passes
   g.tc = g.cols < NORM_THREADS ? g.cols : NORM_THREADS;
   g.rp = NORM_THREADS / g.tc;
-  const long chunks = (g.cols + g.tc - 1) / g.tc;
-  // about four blocks an SM over all pictures, each with at least four rows a thread
-  long s = (4L * sms + g.n * chunks - 1) / (g.n * chunks);
+  g.chunks = (g.cols + g.tc - 1) / g.tc;
+  g.slots = g.groups + g.chunks - 1;
+  const double picture = (double)g.l * g.c * es * bufs;
+  p.pictures = g.n;
+  if (picture * g.n > 80e6 && picture <= 72e6) p.pictures = picture <= 36e6 ? (long)(72e6 / picture) : 1;
+  // the blocks of one launch just fill the SMs, two on each; four rows a thread or more
+  long s = 2L * sms / (p.pictures * g.chunks);
   const long most = (g.l + 4L * g.rp - 1) / (4L * g.rp);
   s = s < most ? s : most;
   g.splits = (int)(s < 1 ? 1 : s);
+  p.part = (size_t)g.n * g.splits * g.slots;
+  p.cpart = grad ? (size_t)g.n * g.splits * g.c : 0;
+  p.g = g;
+  return p;
 }
 
-// Workspace: one (mean, M2) or (sum, sum) per picture, split and channel, the pictures'
-// joined sums, and mean and rstd for callers that do not ask for them. Sized for any
-// vector width: a narrower one has fewer splits, never more.
-long norm_most_splits(long n, long l, int sms) {
-  long s = (4L * sms + n - 1) / n;
-  const long most = (l + 3) / 4;
-  s = s < most ? s : most;
-  return s < 1 ? 1 : s;
-}
+// Workspace for either direction, any element type and vector width.
 size_t norm_work_bytes(long n, long l, int c, int groups, int sms) {
-  return (size_t)n * norm_most_splits(n, l, sms) * c * 8 + (size_t)n * c * 8 + (size_t)n * groups * 8 + 256;
+  size_t most = 0;
+  for (int es = 2; es <= 4; es += 2)
+    for (int vec = 1; vec <= 16 / es; vec *= 2) {
+      if (c % vec) break;
+      for (int grad = 0; grad < 2; ++grad) {
+        NormGeom g{};
+        g.n = n;
+        g.l = l;
+        g.c = c;
+        g.groups = groups;
+        const NormPlan p = norm_plan(g, vec, es, grad, sms);
+        if (p.part + p.cpart > most) most = p.part + p.cpart;
+      }
+    }
+  return most * sizeof(float2);
 }
 
 int norm_check(const char* op, int dtype, int64_t n, int64_t l, int c, int groups, int act) {
@@ -89,65 +139,129 @@ int norm_check(const char* op, int dtype, int64_t n, int64_t l, int c, int group
   return SCB_OK;
 }
 
-// The widest access that every row of every tensor allows.
-int norm_vec(int es, int c, std::initializer_list<uint64_t> bytes) {
-  const int a = common_alignment(16, bytes);
+// The widest access that every row of every tensor allows: `most` bytes, two elements, one.
+int norm_vec(int es, int c, int most, std::initializer_list<uint64_t> bytes) {
+  const int a = common_alignment(most, bytes);
   int v = a / es;
   if (v < 1) return 0;
   while (v > 1 && c % v) v /= 2;
-  return v == 16 / es ? v : v >= 2 ? 2 : 1;
+  return v == most / es ? v : v >= 2 ? 2 : 1;
+}
+
+// Launch `kernel` so that it may start while the launch before it in the stream ends
+// (it waits for that launch's results itself).
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = a;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// Raises a kernel's shared memory limit, once on each device (`raised`: one per kernel).
+cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& raised) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (raised.load() & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) raised.fetch_or(bit);
+  return e;
+}
+
+struct NormArgs {
+  const void *dy, *x;
+  void* y;
+  float *mean, *rstd;
+  const float *weight, *bias;
+  float *dweight, *dbias;
+  float2 *part, *cpart;
+  cudaStream_t st;
+};
+
+template <typename T, int V, bool GRAD, int kT>
+void norm_small(const NormPlan& p, const NormArgs& a) {
+  const auto kernel = norm_small_kernel<T, V, GRAD, kT>;
+  static std::atomic<uint64_t> raised{0};
+  if (allow_smem((const void*)kernel, 227 * 1024, raised) != cudaSuccess) return;  // reported by launched()
+  kernel<<<dim3((unsigned)p.g.n, (unsigned)p.g.chunks), kT, p.smem, a.st>>>(
+      static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<T*>(a.y), a.mean, a.rstd, a.weight, a.bias,
+      a.dweight, a.dbias, p.cpart ? a.cpart : nullptr, p.g);
 }
 
 template <typename T, int V, int ACT>
-void norm_apply(const NormGeom& g, dim3 grid, const void* x, void* y, const float* mean, const float* rstd,
-                const float* w, const float* b, cudaStream_t st) {
-  norm_apply_kernel<T, V, ACT><<<grid, NORM_THREADS, 0, st>>>(static_cast<const T*>(x), static_cast<T*>(y), mean, rstd,
-                                                              w, b, g);
-}
-
-template <typename T, int V>
-void norm_forward(const NormGeom& g, const void* x, void* y, const float* w, const float* b, float* mean, float* rstd,
-                  float2* part, cudaStream_t st) {
-  const dim3 grid((unsigned)(g.n * g.splits), (unsigned)((g.cols + g.tc - 1) / g.tc));
-  const int smem = NORM_THREADS * 4 * (2 * V + 1);
-  norm_stats_kernel<T, V><<<grid, NORM_THREADS, smem, st>>>(static_cast<const T*>(x), part, g);
-  norm_join_kernel<<<(unsigned)(g.n * g.groups), NORM_THREADS, 0, st>>>(part, mean, rstd, g);
-  if (V * sizeof(T) < 16)
-    norm_apply<T, V, ACT_ANY>(g, grid, x, y, mean, rstd, w, b, st);
-  else if (g.act == ACT_RELU)
-    norm_apply<T, V, ACT_RELU>(g, grid, x, y, mean, rstd, w, b, st);
-  else if (g.act == ACT_GELU)
-    norm_apply<T, V, ACT_GELU>(g, grid, x, y, mean, rstd, w, b, st);
-  else if (g.act == ACT_SILU)
-    norm_apply<T, V, ACT_SILU>(g, grid, x, y, mean, rstd, w, b, st);
-  else
-    norm_apply<T, V, ACT_NONE>(g, grid, x, y, mean, rstd, w, b, st);
+void norm_two_pass(const NormPlan& p, const NormArgs& a) {
+  NormGeom g = p.g;
+  const T* x = static_cast<const T*>(a.x);
+  const size_t stat = sizeof(float2) * ((size_t)g.tc * V / g.cpg + 2);
+  for (g.first = 0; g.first < g.n; g.first += p.pictures) {
+    const long n = g.n - g.first < p.pictures ? g.n - g.first : p.pictures;
+    const dim3 grid((unsigned)(n * g.splits), (unsigned)g.chunks);
+    norm_stats_kernel<T, V><<<grid, NORM_THREADS, NORM_THREADS * 4 * (2 * V + 1), a.st>>>(x, a.part, g);
+    launch_after(norm_apply_kernel<T, V, ACT>, grid, NORM_THREADS, stat, a.st, x, static_cast<T*>(a.y), a.part, a.mean,
+                 a.rstd, a.weight, a.bias, g);
+  }
 }
 
 template <typename T, int V, int ACT>
-void norm_backward_act(const NormGeom& g, const void* dy, const void* x, void* dx, const float* mean,
-                       const float* rstd, const float* w, const float* b, float* dw, float* db, float2* part,
-                       float2* sums, cudaStream_t st) {
-  const dim3 grid((unsigned)(g.n * g.splits), (unsigned)((g.cols + g.tc - 1) / g.tc));
-  const T *d = static_cast<const T*>(dy), *p = static_cast<const T*>(x);
-  norm_grad_sums_kernel<T, V, ACT><<<grid, NORM_THREADS, NORM_THREADS * 8 * V, st>>>(d, p, mean, rstd, w, b, part, g);
-  norm_grad_join_kernel<<<(unsigned)g.c, 32, 0, st>>>(part, sums, dw, db, g);
-  norm_grad_apply_kernel<T, V, ACT><<<grid, NORM_THREADS, 0, st>>>(d, p, static_cast<T*>(dx), mean, rstd, w, b, sums, g);
+void norm_two_pass_grad(const NormPlan& p, const NormArgs& a) {
+  NormGeom g = p.g;
+  const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
+  const size_t stat = sizeof(float2) * ((size_t)g.tc * V / g.cpg + 2);
+  for (g.first = 0; g.first < g.n; g.first += p.pictures) {
+    const long n = g.n - g.first < p.pictures ? g.n - g.first : p.pictures;
+    const dim3 grid((unsigned)(n * g.splits), (unsigned)g.chunks);
+    norm_grad_sums_kernel<T, V, ACT><<<grid, NORM_THREADS, NORM_THREADS * 8 * V + stat, a.st>>>(
+        dy, x, a.mean, a.rstd, a.weight, a.bias, a.part, a.cpart, g);
+    launch_after(norm_grad_apply_kernel<T, V, ACT>, grid, NORM_THREADS, 2 * stat, a.st, dy, x, static_cast<T*>(a.y),
+                 a.mean, a.rstd, a.weight, a.bias, a.part, g);
+  }
+}
+
+void norm_params(const NormPlan& p, const NormArgs& a) {
+  if (p.cpart && (a.dweight || a.dbias))
+    norm_grad_params_kernel<<<(unsigned)((p.g.c + 31) / 32), 256, 0, a.st>>>(
+        a.cpart, p.g.n * p.g.splits, p.g.c, a.dweight, a.dbias);
 }
 
 template <typename T, int V>
-void norm_backward(const NormGeom& g, const void* dy, const void* x, void* dx, const float* mean, const float* rstd,
-                   const float* w, const float* b, float* dw, float* db, float2* part, float2* sums, cudaStream_t st) {
-  if (V * sizeof(T) < 16)
-    norm_backward_act<T, V, ACT_ANY>(g, dy, x, dx, mean, rstd, w, b, dw, db, part, sums, st);
-  else if (g.act == ACT_RELU)
-    norm_backward_act<T, V, ACT_RELU>(g, dy, x, dx, mean, rstd, w, b, dw, db, part, sums, st);
-  else if (g.act == ACT_GELU)
-    norm_backward_act<T, V, ACT_GELU>(g, dy, x, dx, mean, rstd, w, b, dw, db, part, sums, st);
-  else if (g.act == ACT_SILU)
-    norm_backward_act<T, V, ACT_SILU>(g, dy, x, dx, mean, rstd, w, b, dw, db, part, sums, st);
+void norm_forward(const NormPlan& p, const NormArgs& a) {
+  if (p.small)
+    p.threads == 128 ? norm_small<T, V, false, 128>(p, a) : norm_small<T, V, false, 512>(p, a);
+  else if (V * sizeof(T) < 16)
+    norm_two_pass<T, V, ACT_ANY>(p, a);
+  else if (p.g.act == ACT_RELU)
+    norm_two_pass<T, V, ACT_RELU>(p, a);
+  else if (p.g.act == ACT_GELU)
+    norm_two_pass<T, V, ACT_GELU>(p, a);
+  else if (p.g.act == ACT_SILU)
+    norm_two_pass<T, V, ACT_SILU>(p, a);
   else
-    norm_backward_act<T, V, ACT_NONE>(g, dy, x, dx, mean, rstd, w, b, dw, db, part, sums, st);
+    norm_two_pass<T, V, ACT_NONE>(p, a);
+}
+
+template <typename T, int V>
+void norm_backward(const NormPlan& p, const NormArgs& a) {
+  if (p.small)
+    p.threads == 128 ? norm_small<T, V, true, 128>(p, a) : norm_small<T, V, true, 512>(p, a);
+  else if (V < 4)
+    norm_two_pass_grad<T, V, ACT_ANY>(p, a);
+  else if (p.g.act == ACT_RELU)
+    norm_two_pass_grad<T, V, ACT_RELU>(p, a);
+  else if (p.g.act == ACT_GELU)
+    norm_two_pass_grad<T, V, ACT_GELU>(p, a);
+  else if (p.g.act == ACT_SILU)
+    norm_two_pass_grad<T, V, ACT_SILU>(p, a);
+  else
+    norm_two_pass_grad<T, V, ACT_NONE>(p, a);
+  norm_params(p, a);
 }
 
 // ---------------------------------------------------------------------------- attention
@@ -227,31 +341,26 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
                    cudaStream_t st) {
   const auto kernel = attn_tc_kernel<T, Boxes>;
   constexpr int smem = AtLayout<Boxes>::kSmem;
-  // the kernel's shared memory limit is raised once on each device
   static std::atomic<uint64_t> raised{0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(raised.load() & bit)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
-    raised.fetch_or(bit);
-  }
+  const cudaError_t e = allow_smem((const void*)kernel, smem, raised);
+  if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
   kernel<<<p.grid, AT_THREADS, smem, st>>>(tk, tv, g);
   if (p.cut || p.twin) attn_join_kernel<T><<<(unsigned)(p.units * (p.unit_rows / 32)), AT_JOIN, 0, st>>>(g, p.grid);
   return launched("scb_attention");
 }
 
-// f<T, V>() for the element type and vector width.
-#define NORM_DISPATCH(dtype, vec, F, ...)                                        \
-  do {                                                                           \
-    if (dtype == SCB_F32)                                                        \
-      vec == 4 ? F<float, 4>(__VA_ARGS__) : vec == 2 ? F<float, 2>(__VA_ARGS__) : F<float, 1>(__VA_ARGS__); \
-    else if (dtype == SCB_F16)                                                   \
-      vec == 8 ? F<__half, 8>(__VA_ARGS__) : vec == 2 ? F<__half, 2>(__VA_ARGS__) : F<__half, 1>(__VA_ARGS__); \
-    else                                                                         \
-      vec == 8 ? F<__nv_bfloat16, 8>(__VA_ARGS__)                                \
-               : vec == 2 ? F<__nv_bfloat16, 2>(__VA_ARGS__) : F<__nv_bfloat16, 1>(__VA_ARGS__); \
+// F<T, V>() for the element type and vector width; the gradient keeps more of each channel in
+// registers and takes 16-bit types four at a time.
+#define NORM_TYPED(T, wide, vec, F, ...) \
+  (vec == wide ? F<T, wide>(__VA_ARGS__) : vec == 2 ? F<T, 2>(__VA_ARGS__) : F<T, 1>(__VA_ARGS__))
+#define NORM_DISPATCH(dtype, wide16, vec, F, ...)                       \
+  do {                                                                  \
+    if (dtype == SCB_F32)                                               \
+      NORM_TYPED(float, 4, vec, F, __VA_ARGS__);                        \
+    else if (dtype == SCB_F16)                                          \
+      NORM_TYPED(__half, wide16, vec, F, __VA_ARGS__);                  \
+    else                                                                \
+      NORM_TYPED(__nv_bfloat16, wide16, vec, F, __VA_ARGS__);           \
   } while (0)
 
 }  // namespace
@@ -285,23 +394,24 @@ int scb_group_norm(const void* x, int64_t x_sn, int64_t x_sl, int dtype, int64_t
     if (!(eps >= 0.f)) return refuse(op, "eps must not be negative");
     const int es = elem_size(dtype), sms = sm_count();
     if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
-    if (!work || work_bytes < norm_work_bytes(n, l, c, groups, sms) || addr(work) % 16)
+    const size_t need = norm_work_bytes(n, l, c, groups, sms);
+    if (need && (!work || work_bytes < need || addr(work) % 16))
       return refuse(op, "the workspace is too small or not 16-byte aligned (scb_group_norm_workspace)");
     if ((mean && addr(mean) % 4) || (rstd && addr(rstd) % 4) || addr(weight) % 4 || addr(bias) % 4)
       return refuse(op, "misaligned float pointer");
-    const int vec = norm_vec(es, c, {addr(x), addr(y), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
+    const int vec = norm_vec(es, c, 16, {addr(x), addr(y), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
                                      (uint64_t)(y_sn * es), (uint64_t)(y_sl * es)});
     if (!vec) return refuse(op, "data not aligned to its element size");
     NormGeom g{};
     g.n = n; g.l = l; g.c = c; g.groups = groups; g.eps = eps; g.act = act;
     g.x_sn = x_sn; g.x_sl = x_sl; g.y_sn = y_sn; g.y_sl = y_sl;
-    norm_plan(g, vec, sms);
-    if (g.n * g.splits > kMaxBlocks || n * groups > kMaxBlocks) return refuse(op, "too many pictures");
-    float2* part = static_cast<float2*>(work);
-    float* own = reinterpret_cast<float*>(part + (size_t)n * g.splits * c);
-    if (!mean) mean = own;
-    if (!rstd) rstd = own + (size_t)n * groups;
-    NORM_DISPATCH(dtype, vec, norm_forward, g, x, y, weight, bias, mean, rstd, part, static_cast<cudaStream_t>(stream));
+    const NormPlan p = norm_plan(g, vec, es, false, sms);
+    if (n * p.g.splits > kMaxBlocks || p.g.chunks > 65535) return refuse(op, "too many pictures or channels");
+    NormArgs a{};
+    a.x = x; a.y = y; a.mean = mean; a.rstd = rstd; a.weight = weight; a.bias = bias;
+    a.part = static_cast<float2*>(work);
+    a.st = static_cast<cudaStream_t>(stream);
+    NORM_DISPATCH(dtype, 8, vec, norm_forward, p, a);
     return launched(op);
   });
 }
@@ -326,20 +436,25 @@ int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const vo
       return refuse(op, "negative input strides or overlapping output rows");
     const int es = elem_size(dtype), sms = sm_count();
     if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
-    if (!work || work_bytes < norm_work_bytes(n, l, c, groups, sms) || addr(work) % 16)
+    const size_t need = norm_work_bytes(n, l, c, groups, sms);
+    if (need && (!work || work_bytes < need || addr(work) % 16))
       return refuse(op, "the workspace is too small or not 16-byte aligned (scb_group_norm_workspace)");
-    const int vec = norm_vec(es, c, {addr(x), addr(dy), addr(dx), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
+    const int vec = norm_vec(es, c, es == 2 ? 8 : 16, {addr(x), addr(dy), addr(dx), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
                                      (uint64_t)(d_sn * es), (uint64_t)(d_sl * es), (uint64_t)(dx_sn * es),
                                      (uint64_t)(dx_sl * es)});
     if (!vec) return refuse(op, "data not aligned to its element size");
     NormGeom g{};
     g.n = n; g.l = l; g.c = c; g.groups = groups; g.act = act;
     g.x_sn = x_sn; g.x_sl = x_sl; g.y_sn = dx_sn; g.y_sl = dx_sl; g.d_sn = d_sn; g.d_sl = d_sl;
-    norm_plan(g, vec, sms);
-    if (g.n * g.splits > kMaxBlocks) return refuse(op, "too many pictures");
-    float2* part = static_cast<float2*>(work);
-    float2* sums = part + (size_t)n * g.splits * c;
-    NORM_DISPATCH(dtype, vec, norm_backward, g, dy, x, dx, mean, rstd, weight, bias, dweight, dbias, part, sums, st);
+    const NormPlan p = norm_plan(g, vec, es, true, sms);
+    if (n * p.g.splits > kMaxBlocks || p.g.chunks > 65535) return refuse(op, "too many pictures or channels");
+    NormArgs a{};
+    a.dy = dy; a.x = x; a.y = dx; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+    a.weight = weight; a.bias = bias; a.dweight = dweight; a.dbias = dbias;
+    a.part = static_cast<float2*>(work);
+    a.cpart = a.part + p.part;
+    a.st = st;
+    NORM_DISPATCH(dtype, 4, vec, norm_backward, p, a);
     return launched(op);
   });
 }
@@ -391,25 +506,70 @@ int scb_rotate_axes(const scb_heads* q, const scb_heads* k, int dtype, int64_t b
     g.pos = pos; g.pos_sb = pos_sb; g.pos_sl = pos_sl; g.pos_sa = pos_sa;
     g.freq = inv_freq;
     g.sign = inverse ? -1.f : 1.f;
-    g.per_block = 8;
-    while (g.per_block > 1 && g.per_block * g.pairs > 4096) g.per_block /= 2;
+    if (l >= 0x7fff0000) return refuse(op, "too many tokens");
     if (g.pairs > 4096) return refuse(op, "heads wider than 8192 channels");
+    // the widest vector that the sections, the strides and the addresses allow
+    int vec = 16 / es;
+    uint64_t bytes = 0;
+    for (const RotTensor& t : g.t) {
+      if (!t.heads) continue;
+      bytes |= addr(t.x) | addr(t.y);
+      for (int64_t s : {t.x_sb, t.x_sl, t.x_sh, t.y_sb, t.y_sl, t.y_sh}) bytes |= (uint64_t)s * es;
+    }
+    const auto splits = [&](int v) {
+      if (layout == ROT_INTERLEAVED) return d % (2 * v) == 0;
+      if (d % v || g.pairs % v) return false;
+      if (layout == ROT_AXIAL)
+        for (int a = 1; a <= axes; ++a)
+          if (g.first[a] % v) return false;
+      return true;
+    };
+    while (vec > 1 && (bytes % (uint64_t)(vec * es) || !splits(vec))) vec /= 2;
+    g.vecs = layout == ROT_INTERLEAVED && vec > 1 ? d / 2 / vec : (d - g.pairs) / vec;
+    g.items = (unsigned)g.vecs * (unsigned)(g.t[0].heads + g.t[1].heads);
+    if (!g.items) return SCB_OK;
+    if ((uint64_t)g.vecs * (uint64_t)(g.t[0].heads + g.t[1].heads) > 1u << 24) return refuse(op, "heads too many or too wide");
+    // tokens of a block: four items a thread, but blocks for every SM; angles of at most 32 KB
+    long per = (4L * ROT_THREADS + g.items - 1) / g.items;
+    const int sms = sm_count();
+    if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
+    const long share = (g.tokens + 2L * sms - 1) / (2L * sms);
+    per = per < share ? per : share;
+    per = per * g.pairs > 4096 ? 4096 / g.pairs : per;
+    g.per_block = (int)(per < 1 ? 1 : per);
+    g.by_items = Divide::by(g.items);
+    g.by_vecs = Divide::by((unsigned)g.vecs);
+    g.by_l = Divide::by((unsigned)l);
+    g.by_pairs = Divide::by((unsigned)g.pairs);
     const long blocks = (g.tokens + g.per_block - 1) / g.per_block;
     if (blocks > kMaxBlocks) return refuse(op, "too many tokens");
     const int smem = g.per_block * g.pairs * (int)sizeof(float2);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define ROT_LAYOUTS(T)                                                                            \
-  (layout == ROT_HALF ? rotary_kernel<T, ROT_HALF><<<(unsigned)blocks, ROT_THREADS, smem, st>>>(g) \
-   : layout == ROT_INTERLEAVED                                                                    \
-       ? rotary_kernel<T, ROT_INTERLEAVED><<<(unsigned)blocks, ROT_THREADS, smem, st>>>(g)        \
-       : rotary_kernel<T, ROT_AXIAL><<<(unsigned)blocks, ROT_THREADS, smem, st>>>(g))
-    if (dtype == SCB_F32)
-      ROT_LAYOUTS(float);
-    else if (dtype == SCB_F16)
-      ROT_LAYOUTS(__half);
-    else
-      ROT_LAYOUTS(__nv_bfloat16);
+    const auto launch = [&](auto kernel) { kernel<<<(unsigned)blocks, ROT_THREADS, smem, st>>>(g); };
+#define ROT_VECS(T, L)                                        \
+  switch (vec) {                                              \
+    case 8: launch(rotary_kernel<T, L, 16 / sizeof(T)>); break; \
+    case 4: launch(rotary_kernel<T, L, 4>); break;            \
+    case 2: launch(rotary_kernel<T, L, 2>); break;            \
+    default: launch(rotary_kernel<T, L, 1>);                  \
+  }
+#define ROT_LAYOUTS(T)                                              \
+  if (layout == ROT_HALF) {                                         \
+    ROT_VECS(T, ROT_HALF)                                           \
+  } else if (layout == ROT_INTERLEAVED) {                           \
+    ROT_VECS(T, ROT_INTERLEAVED)                                    \
+  } else {                                                          \
+    ROT_VECS(T, ROT_AXIAL)                                          \
+  }
+    if (dtype == SCB_F32) {
+      ROT_LAYOUTS(float)
+    } else if (dtype == SCB_F16) {
+      ROT_LAYOUTS(__half)
+    } else {
+      ROT_LAYOUTS(__nv_bfloat16)
+    }
 #undef ROT_LAYOUTS
+#undef ROT_VECS
     return launched(op);
   });
 }

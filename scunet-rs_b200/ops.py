@@ -113,7 +113,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act="none", out=N
             mean, rstd = (torch.empty((n, max(groups, 1)), dtype=torch.float32, device=x.device) for _ in range(2))
         work = _workspace(lib.scb_group_norm_workspace, lib, x.device, n, l, c, groups)
         _check(lib.scb_group_norm(x.data_ptr(), sn, sl, dt, n, l, c, groups, w, b, eps, SCB_ACTS[act], out.data_ptr(),
-                                  on, ol, _ptr(mean), _ptr(rstd), _ptr(work), work.numel() if n else 0, _stream(x)), lib)
+                                  on, ol, _ptr(mean), _ptr(rstd), _ptr(work), 0 if work is None else work.numel(), _stream(x)), lib)
     return (out, mean, rstd) if stats else out
 
 
@@ -142,7 +142,7 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, ac
         work = _workspace(lib.scb_group_norm_workspace, lib, x.device, n, l, c, groups)
         _check(lib.scb_group_norm_backward(dy.data_ptr(), dn, dl, x.data_ptr(), sn, sl, dt, n, l, c, groups,
                                            mean.data_ptr(), rstd.data_ptr(), w, b, SCB_ACTS[act], out.data_ptr(), on,
-                                           ol, dw.data_ptr(), db.data_ptr(), _ptr(work), work.numel() if n else 0,
+                                           ol, dw.data_ptr(), db.data_ptr(), _ptr(work), 0 if work is None else work.numel(),
                                            _stream(x)), lib)
     return out, dw, db
 
