@@ -28,7 +28,10 @@ struct Dim {
 template <size_t N>
 bool distinct_elements(int64_t inner, const Dim (&given)[N]) {
   Dim d[N];
-  for (size_t i = 0; i < N; ++i) d[i] = given[i];
+  for (size_t i = 0; i < N; ++i) {
+    d[i] = given[i];
+    if (d[i].size == 0) return true;
+  }
   for (size_t i = 1; i < N; ++i)  // insertion sort by stride
     for (size_t j = i; j > 0 && d[j].stride < d[j - 1].stride; --j) {
       const Dim t = d[j];

@@ -17,10 +17,9 @@
 //    read last is still in L2.
 // A thread keeps its channels (a vector of up to 16 bytes) and steps over rows.
 //
-// Statistics are fp32: a thread sums x - K and (x - K)^2 with K its first value of the
-// channel, so that the sum of squares loses nothing to a large mean (K is one of the
-// values, so a K far from the rest is itself part of the spread it stands against), and
-// (count, mean, M2) triples are joined pairwise,
+// Statistics are fp32: a block sums x - K and (x - K)^2 with K the median of the channel's
+// values in its first, middle and last row, so that the sum of squares loses nothing to a
+// large mean or to one value far from the rest, and (count, mean, M2) triples are joined,
 //   M2 = M2a + M2b + (mb - ma)^2 na nb / (na + nb).
 // No atomics: the order of every sum is fixed by the sizes.
 #pragma once
@@ -37,15 +36,16 @@ struct NormGeom {
   int chunks, slots;  // chunks of a row; groups + chunks - 1 partials of a split: a chunk's
                       // part of a group is slot group + chunk (a group may span chunks)
   int splits;         // row ranges of a picture
+  int whole;          // a vector never spans two groups
   long x_sn, x_sl;    // element strides of pictures and rows
   long y_sn, y_sl;
   long d_sn, d_sl;    // dy
   float eps;
   int act;            // read by the kernels compiled for ACT_ANY
+  int keep;           // small form: where the values start in shared memory, in floats
 };
 
 constexpr int NORM_THREADS = 512;  // two blocks an SM: every block reads its picture's partials
-constexpr int NORM_SMALL_BYTES = 184 * 1024;  // shared memory for the small form's values
 
 struct Moments {
   float n, mean, m2;
@@ -53,7 +53,7 @@ struct Moments {
 __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
   const float n = a.n + b.n;
   if (n == 0.f) return a;
-  const float d = b.mean - a.mean, f = b.n / n;
+  const float d = b.mean - a.mean, f = __fdividef(b.n, n);
   return {n, a.mean + d * f, a.m2 + b.m2 + d * d * a.n * f};
 }
 __device__ __forceinline__ Moments shfl_xor(const Moments& m, int d) {
@@ -143,6 +143,12 @@ __device__ __forceinline__ void slope_all(const NormGeom& g, float* z) {
   }
 }
 
+// The group of channel c0 + i: one division for a thread's vector when the groups are whole
+// vectors.
+__device__ __forceinline__ int group_of(const NormGeom& g, int c0, int i) {
+  return g.whole ? c0 / g.cpg : (c0 + i) / g.cpg;
+}
+
 // What a thread needs of its channels: z = x sc + sh (one rounding; sh holds b - mean sc,
 // whose rounding is that of the mean itself).
 template <int V>
@@ -153,7 +159,7 @@ struct Channels {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = c0 + i;
-      const float2 st = stats[c / g.cpg - first_group];
+      const float2 st = stats[group_of(g, c0, i) - first_group];
       sc[i] = st.y * (weight ? weight[c] : 1.f);
       sh[i] = fmaf(-st.x, sc[i], bias ? bias[c] : 0.f);
     }
@@ -170,7 +176,7 @@ struct Hats {
   __device__ __forceinline__ void load(const NormGeom& g, const float2* stats, int first_group, int c0) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float2 st = stats[(c0 + i) / g.cpg - first_group];
+      const float2 st = stats[group_of(g, c0, i) - first_group];
       rs[i] = st.y;
       mr[i] = -st.x * st.y;
     }
@@ -178,87 +184,101 @@ struct Hats {
   __device__ __forceinline__ float at(int i, float x) const { return fmaf(x, rs[i], mr[i]); }
 };
 
-// The running sums of a thread, joined over the block's row lanes in shared memory.
-template <int V>
-struct RowMoments {
-  float k[V], s[V], q[V], cnt;
-  __device__ __forceinline__ void clear() {
-    cnt = 0.f;
+// A block's sums of two values per channel over its row lanes. Every thread leaves its V
+// channels' sums; (segment, channel) threads add some lanes each; `at` adds the segments.
+// Memory: [lanes][channels] of each value, then [segments][channels] of each.
+template <int V, int T>
+struct BlockSums {
+  __host__ __device__ static int floats(int tc) { return 2 * V * T + 2 * (tc * V > T ? tc * V : T); }
+  float *a, *b, *sa, *sb;
+  int channels, segs;
+  __device__ __forceinline__ void add(float* mem, const NormGeom& g, const float* va, const float* vb, int lane) {
+    channels = g.tc * V;
+    segs = min(g.rp, T / channels);
+    segs = segs < 1 ? 1 : segs;
+    a = mem;
+    b = mem + V * T;
+    sa = mem + 2 * V * T;
+    sb = sa + max(T, channels);
+    const int t = threadIdx.x - lane * g.tc;
+    if (lane < g.rp) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) k[i] = s[i] = q[i] = 0.f;
-  }
-  __device__ __forceinline__ void start(const float* v) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) k[i] = v[i];
-  }
-  __device__ __forceinline__ void add(const float* v) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float d = v[i] - k[i];
-      s[i] += d;
-      q[i] += d * d;
+      for (int i = 0; i < V; ++i) {
+        a[lane * channels + t * V + i] = va[i];
+        b[lane * channels + t * V + i] = vb[i];
+      }
     }
+    __syncthreads();
+    for (int k = threadIdx.x; k < segs * channels; k += T) {
+      const int seg = k / channels, ch = k - seg * channels;
+      float xa = 0.f, xb = 0.f;
+      for (int r = seg; r < g.rp; r += segs) {
+        xa += a[r * channels + ch];
+        xb += b[r * channels + ch];
+      }
+      sa[k] = xa;
+      sb[k] = xb;
+    }
+    __syncthreads();
   }
-  static constexpr int kFloats = 2 * V + 1;  // per thread
+  __device__ __forceinline__ float2 at(int ch) const {
+    float xa = 0.f, xb = 0.f;
+    for (int k = 0; k < segs; ++k) {
+      xa += sa[k * channels + ch];
+      xb += sb[k * channels + ch];
+    }
+    return make_float2(xa, xb);
+  }
 };
 
-// Joins the row lanes' moments per channel into lane 0's places: mean at mem[i * T + t],
-// M2 at mem[(V + i) * T + t] for channel t V + i of the chunk.
-template <int V, int T>
-__device__ __forceinline__ void join_lanes(const RowMoments<V>& r, float* mem, int tc, int rp, int lane) {
-  const int tid = threadIdx.x;
-  float *sm = mem, *sq = mem + V * T, *sn = mem + 2 * V * T;
-  const float inv = r.cnt > 0.f ? 1.f / r.cnt : 0.f;
-  sn[tid] = r.cnt;
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    sm[i * T + tid] = r.k[i] + r.s[i] * inv;
-    sq[i * T + tid] = r.cnt > 0.f ? fmaxf(r.q[i] - r.s[i] * r.s[i] * inv, 0.f) : 0.f;
-    if (r.q[i] != r.q[i]) sq[i * T + tid] = r.q[i];  // fmaxf would drop a NaN
-  }
-  int top = 1;
-  while (top < rp) top *= 2;
-  for (int h = top / 2; h >= 1; h /= 2) {
-    __syncthreads();
-    if (lane < h && lane + h < rp) {
-      const int o = tid + h * tc;
-      const float na = sn[tid], nb = sn[o];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int a = i * T;
-        const Moments m = join(Moments{na, sm[a + tid], sq[a + tid]}, Moments{nb, sm[a + o], sq[a + o]});
-        sm[a + tid] = m.mean;
-        sq[a + tid] = m.m2;
-      }
-      sn[tid] = na + nb;
-    }
-  }
-  __syncthreads();
+  for (int d = 16; d >= 1; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
 }
-// The same for two plain sums.
+
+// Mean and M2 of channels [lo, hi) of a chunk over `rows` rows, by one warp: the channels'
+// means average to the group's, M2 = sum (M2_c + rows (mean_c - mean)^2).
 template <int V, int T>
-__device__ __forceinline__ void add_lanes(const float* a, const float* b, float* mem, int tc, int rp, int lane) {
-  const int tid = threadIdx.x;
-  float *ra = mem, *rb = mem + V * T;
+__device__ __forceinline__ float2 group_moments(const BlockSums<V, T>& s, const float* first, int lo, int hi,
+                                                float rows) {
+  const int lane = threadIdx.x & 31;
+  const float inv = rows > 0.f ? 1.f / rows : 0.f;
+  float mean = 0.f;
+  for (int ch = lo + lane; ch < hi; ch += 32) mean += first[ch] + s.at(ch).x * inv;
+  mean = warp_sum(mean) / (float)(hi - lo);
+  float m2 = 0.f;
+  for (int ch = lo + lane; ch < hi; ch += 32) {
+    const float2 v = s.at(ch);
+    const float d = first[ch] + v.x * inv - mean, own = v.y - v.x * v.x * inv;
+    m2 += (own < 0.f ? 0.f : own) + rows * d * d;  // (a NaN stays)
+  }
+  return make_float2(mean, warp_sum(m2));
+}
+
+// The channels' K for rows [r0, r1) of a block.
+template <typename T, int V>
+__device__ __forceinline__ void middle_of_rows(const T* src, long stride, long r0, long r1, float* k) {
+  Pack<T, V> a, b, c;
+  a.load(src + r0 * stride);
+  b.load(src + (r0 + (r1 - r0) / 2) * stride);
+  c.load(src + (r1 - 1) * stride);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    ra[i * T + tid] = a[i];
-    rb[i * T + tid] = b[i];
+    const float x = to_f32(a.v[i]), y = to_f32(b.v[i]), z = to_f32(c.v[i]);
+    k[i] = fmaxf(fminf(x, y), fminf(fmaxf(x, y), z));
   }
-  int top = 1;
-  while (top < rp) top *= 2;
-  for (int h = top / 2; h >= 1; h /= 2) {
-    __syncthreads();
-    if (lane < h && lane + h < rp) {
-      const int o = tid + h * tc;
+}
+
+// s += v - k, q += (v - k)^2
+template <int V>
+__device__ __forceinline__ void add_moments(const float* v, const float* k, float* s, float* q) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        ra[i * T + tid] += ra[i * T + o];
-        rb[i * T + tid] += rb[i * T + o];
-      }
-    }
+  for (int i = 0; i < V; ++i) {
+    const float d = v[i] - k[i];
+    s[i] += d;
+    q[i] = fmaf(d, d, q[i]);
   }
-  __syncthreads();
 }
 
 // The row range of split s.
@@ -295,38 +315,36 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 template <typename T, int V>
 __global__ void __launch_bounds__(NORM_THREADS, 2)
 norm_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, const __grid_constant__ NormGeom g) {
-  extern __shared__ float norm_sm[];
+  extern __shared__ __align__(16) float norm_sm[];
   let_next_start();
   const NormPlace p(g, V);
-  RowMoments<V> r;
-  r.clear();
-  long row = p.r0 + p.lane;
-  if (p.on && row < p.r1) {
+  float k[V], sum[V], sq[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) k[i] = sum[i] = sq[i] = 0.f;
+  float* first = norm_sm + BlockSums<V, NORM_THREADS>::floats(g.tc);  // K of the chunk's channels
+  if (p.on && p.r0 < p.r1) {
     const T* src = x + p.pic * g.x_sn + (long)p.col * V;
     Pack<T, V> a;
     float v[V];
-    a.load(src + row * g.x_sl);
-    unpack(a, v);
-    r.start(v);
-    r.cnt = (float)((p.r1 - row + g.rp - 1) / g.rp);
+    middle_of_rows<T, V>(src, g.x_sl, p.r0, p.r1, k);
 #pragma unroll 4
-    for (; row < p.r1; row += g.rp) {
+    for (long row = p.r0 + p.lane; row < p.r1; row += g.rp) {
       a.load(src + row * g.x_sl);
       unpack(a, v);
-      r.add(v);
+      add_moments<V>(v, k, sum, sq);
     }
   }
-  join_lanes<V, NORM_THREADS>(r, norm_sm, g.tc, g.rp, p.lane);
-  const float rows = (float)(p.r1 - p.r0);
+  if (p.lane == 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) first[threadIdx.x * V + i] = k[i];
+  }
+  BlockSums<V, NORM_THREADS> sums;
+  sums.add(norm_sm, g, sum, sq, p.lane);
   float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
   for (int grp = p.c0 / g.cpg + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
-    Moments m{0.f, 0.f, 0.f};
-    for (int c = max(grp * g.cpg, p.c0) + (threadIdx.x & 31); c < min((grp + 1) * g.cpg, p.c1); c += 32) {
-      const int e = c - p.c0, at = (e % V) * NORM_THREADS + e / V;
-      m = join(m, Moments{rows, norm_sm[at], norm_sm[V * NORM_THREADS + at]});
-    }
-    m = warp_join(m);
-    if ((threadIdx.x & 31) == 0) out[grp] = make_float2(m.mean, m.m2);
+    const float2 m = group_moments(sums, first, max(grp * g.cpg, p.c0) - p.c0, min((grp + 1) * g.cpg, p.c1) - p.c0,
+                                   (float)(p.r1 - p.r0));
+    if ((threadIdx.x & 31) == 0) out[grp] = m;
   }
 }
 
@@ -354,7 +372,7 @@ __global__ void __launch_bounds__(NORM_THREADS, 2)
 norm_apply_kernel(const T* x, T* y, const float2* __restrict__ part,
                   float* __restrict__ mean, float* __restrict__ rstd, const float* __restrict__ weight,
                   const float* __restrict__ bias, const __grid_constant__ NormGeom g) {
-  extern __shared__ float2 norm_stat[];  // of the chunk's groups
+  extern __shared__ __align__(16) float2 norm_stat[];  // of the chunk's groups
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg;
   wait_for_previous();
@@ -433,11 +451,11 @@ norm_grad_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const f
                       const float* __restrict__ rstd, const float* __restrict__ weight,
                       const float* __restrict__ bias, float2* __restrict__ part, float2* __restrict__ cpart,
                       const __grid_constant__ NormGeom g) {
-  extern __shared__ float norm_sm[];  // [2][V][threads], then the chunk's groups' statistics
+  extern __shared__ __align__(16) float norm_sm[];  // the block's sums, then the chunk's groups' statistics
   let_next_start();
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg;
-  float2* stats = reinterpret_cast<float2*>(norm_sm + 2 * V * NORM_THREADS);
+  float2* stats = reinterpret_cast<float2*>(norm_sm + BlockSums<V, NORM_THREADS>::floats(g.tc));
   grad_stats(g, stats, g0, p.c1, mean, rstd, p.pic);
   __syncthreads();
   float sa[V], sb[V];
@@ -458,14 +476,14 @@ norm_grad_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const f
       add_grad<T, V, ACT>(g, ch, hat, a, e, sa, sb);
     }
   }
-  add_lanes<V, NORM_THREADS>(sa, sb, norm_sm, g.tc, g.rp, p.lane);
+  BlockSums<V, NORM_THREADS> sums;
+  sums.add(norm_sm, g, sa, sb, p.lane);
   float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
   float2* cout = cpart + (p.pic * g.splits + p.split) * g.c;
   for (int grp = g0 + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
     float2 m = make_float2(0.f, 0.f);
     for (int c = max(grp * g.cpg, p.c0) + (threadIdx.x & 31); c < min((grp + 1) * g.cpg, p.c1); c += 32) {
-      const int e = c - p.c0, at = (e % V) * NORM_THREADS + e / V;
-      const float2 s = make_float2(norm_sm[at], norm_sm[V * NORM_THREADS + at]);
+      const float2 s = sums.at(c - p.c0);
       cout[c] = s;
       const float w = weight ? weight[c] : 1.f;
       m = join(m, make_float2(w * s.x, w * s.y));
@@ -494,7 +512,7 @@ struct GradMeans {
                                        int c0) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float2 m = means[(c0 + i) / g.cpg - first_group];
+      const float2 m = means[group_of(g, c0, i) - first_group];
       m1[i] = hat.rs[i] * m.x;
       m2[i] = hat.rs[i] * m.y;
     }
@@ -518,7 +536,7 @@ norm_grad_apply_kernel(const T* dy, const T* x, T* dx,
                        const float* __restrict__ mean, const float* __restrict__ rstd,
                        const float* __restrict__ weight, const float* __restrict__ bias,
                        const float2* __restrict__ part, const __grid_constant__ NormGeom g) {
-  extern __shared__ float2 norm_stat[];  // (mean, rstd), then (E[h], E[h xh]) of the chunk's groups
+  extern __shared__ __align__(16) float2 norm_stat[];  // (mean, rstd), then (E[h], E[h xh]) of the chunk's groups
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg, ng = (p.c1 - 1) / g.cpg - g0 + 1;
   grad_stats(g, norm_stat, g0, p.c1, mean, rstd, p.pic);
@@ -584,46 +602,45 @@ norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
                   float* __restrict__ dweight, float* __restrict__ dbias, float2* __restrict__ cpart,
                   const __grid_constant__ NormGeom g) {
   extern __shared__ __align__(16) float norm_sm[];
-  // [2 V + 1][threads] lanes; (mean, rstd), (E[h], E[h xh]) of the groups; the values
-  float2* stats = reinterpret_cast<float2*>(norm_sm + (2 * V + 1) * kT);
+  // the block's sums; K; (mean, rstd), (E[h], E[h xh]) of the groups; the values
+  float* first = norm_sm + BlockSums<V, kT>::floats(g.tc);
+  float2* stats = reinterpret_cast<float2*>(first + (g.tc * V + 1) / 2 * 2);
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg, ng = (p.c1 - p.c0) / g.cpg;
-  Pack<T, V>* keep = reinterpret_cast<Pack<T, V>*>(norm_sm + (2 * V + 1) * kT + 4 * ((g.tc * V / g.cpg + 3) / 4 * 4));
+  Pack<T, V>* keep = reinterpret_cast<Pack<T, V>*>(norm_sm + g.keep);
   Pack<T, V>* keep_d = keep + (GRAD ? g.l * g.tc : 0);
   const int t = threadIdx.x % g.tc;
   const T* src = x + p.pic * g.x_sn + (long)p.col * V;
   const T* del = GRAD ? dy + p.pic * g.d_sn + (long)p.col * V : nullptr;
   if (!GRAD) {
-    RowMoments<V> r;
-    r.clear();
-    if (p.on && p.lane < g.l) {
+    float k[V], sum[V], sq[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) k[i] = sum[i] = sq[i] = 0.f;
+    if (p.on && g.l > 0) {
       Pack<T, V> a;
       float v[V];
-      a.load(src + p.lane * g.x_sl);
-      unpack(a, v);
-      r.start(v);
-      r.cnt = (float)((g.l - p.lane + g.rp - 1) / g.rp);
+      middle_of_rows<T, V>(src, g.x_sl, 0, g.l, k);
 #pragma unroll 4
       for (long row = p.lane; row < g.l; row += g.rp) {
         a.load(src + row * g.x_sl);
         keep[row * g.tc + t] = a;
         unpack(a, v);
-        r.add(v);
+        add_moments<V>(v, k, sum, sq);
       }
     }
-    join_lanes<V, kT>(r, norm_sm, g.tc, g.rp, p.lane);
-    for (int k = threadIdx.x >> 5; k < ng; k += kT / 32) {
-      Moments m{0.f, 0.f, 0.f};
-      for (int e = k * g.cpg + (threadIdx.x & 31); e < (k + 1) * g.cpg; e += 32) {
-        const int at = (e % V) * kT + e / V;
-        m = join(m, Moments{(float)g.l, norm_sm[at], norm_sm[V * kT + at]});
-      }
-      m = warp_join(m);
+    if (p.lane == 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) first[t * V + i] = k[i];
+    }
+    BlockSums<V, kT> sums;
+    sums.add(norm_sm, g, sum, sq, p.lane);
+    for (int n = threadIdx.x >> 5; n < ng; n += kT / 32) {
+      const float2 m = group_moments(sums, first, n * g.cpg, (n + 1) * g.cpg, (float)g.l);
       if ((threadIdx.x & 31) == 0) {
-        const float rs = 1.f / sqrtf((m.n > 0.f ? m.m2 / m.n : 0.f) + g.eps);
-        stats[k] = make_float2(m.mean, rs);
-        if (mean) mean[p.pic * g.groups + g0 + k] = m.mean;
-        if (rstd) rstd[p.pic * g.groups + g0 + k] = rs;
+        const float rs = 1.f / sqrtf((g.l > 0 ? m.y / ((float)g.l * (float)g.cpg) : 0.f) + g.eps);
+        stats[n] = make_float2(m.x, rs);
+        if (mean) mean[p.pic * g.groups + g0 + n] = m.x;
+        if (rstd) rstd[p.pic * g.groups + g0 + n] = rs;
       }
     }
   } else {
@@ -647,46 +664,47 @@ norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
         repack<T, V>(v).store(dst + row * g.y_sl);
       }
   } else {
-  float sa[V], sb[V];
+    float sa[V], sb[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.f;
-  if (p.on) {
+    for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.f;
+    if (p.on) {
 #pragma unroll 2
-    for (long row = p.lane; row < g.l; row += g.rp) {
-      Pack<T, V> a, e;
-      a.load(src + row * g.x_sl);
-      e.load(del + row * g.d_sl);
-      keep[row * g.tc + t] = a;
-      keep_d[row * g.tc + t] = e;
-      add_grad<T, V, ACT_ANY>(g, ch, hat, a, e, sa, sb);
-    }
-  }
-  add_lanes<V, kT>(sa, sb, norm_sm, g.tc, g.rp, p.lane);
-  float2* means = stats + ng;
-  for (int k = threadIdx.x >> 5; k < ng; k += kT / 32) {
-    float2 m = make_float2(0.f, 0.f);
-    for (int e = k * g.cpg + (threadIdx.x & 31); e < (k + 1) * g.cpg; e += 32) {
-      const int at = (e % V) * kT + e / V, c = p.c0 + e;
-      const float2 s = make_float2(norm_sm[at], norm_sm[V * kT + at]);
-      const float w = weight ? weight[c] : 1.f;
-      m = join(m, make_float2(w * s.x, w * s.y));
-      if (cpart) {
-        cpart[p.pic * g.c + c] = s;
-      } else {
-        if (dbias) dbias[c] = s.x;
-        if (dweight) dweight[c] = s.y;
+      for (long row = p.lane; row < g.l; row += g.rp) {
+        Pack<T, V> a, e;
+        a.load(src + row * g.x_sl);
+        e.load(del + row * g.d_sl);
+        keep[row * g.tc + t] = a;
+        keep_d[row * g.tc + t] = e;
+        add_grad<T, V, ACT_ANY>(g, ch, hat, a, e, sa, sb);
       }
     }
-    m = warp_join(m);
-    const float inv = 1.f / ((float)g.l * (float)g.cpg);
-    if ((threadIdx.x & 31) == 0) means[k] = make_float2(m.x * inv, m.y * inv);
-  }
-  __syncthreads();
-  if (!p.on) return;
-  GradMeans<V> m;
-  m.load(g, hat, means, g0, p.col * V);
-  for (long row = p.lane; row < g.l; row += g.rp)
-    grad_x<T, V, ACT_ANY>(g, ch, hat, m, keep[row * g.tc + t], keep_d[row * g.tc + t]).store(dst + row * g.y_sl);
+    BlockSums<V, kT> sums;
+    sums.add(norm_sm, g, sa, sb, p.lane);
+    float2* means = stats + ng;
+    for (int k = threadIdx.x >> 5; k < ng; k += kT / 32) {
+      float2 m = make_float2(0.f, 0.f);
+      for (int e = k * g.cpg + (threadIdx.x & 31); e < (k + 1) * g.cpg; e += 32) {
+        const int c = p.c0 + e;
+        const float2 s = sums.at(e);
+        const float w = weight ? weight[c] : 1.f;
+        m = join(m, make_float2(w * s.x, w * s.y));
+        if (cpart) {
+          cpart[p.pic * g.c + c] = s;
+        } else {
+          if (dbias) dbias[c] = s.x;
+          if (dweight) dweight[c] = s.y;
+        }
+      }
+      m = warp_join(m);
+      const float inv = 1.f / ((float)g.l * (float)g.cpg);
+      if ((threadIdx.x & 31) == 0) means[k] = make_float2(m.x * inv, m.y * inv);
+    }
+    __syncthreads();
+    if (!p.on) return;
+    GradMeans<V> m;
+    m.load(g, hat, means, g0, p.col * V);
+    for (long row = p.lane; row < g.l; row += g.rp)
+      grad_x<T, V, ACT_ANY>(g, ch, hat, m, keep[row * g.tc + t], keep_d[row * g.tc + t]).store(dst + row * g.y_sl);
   }
 }
 

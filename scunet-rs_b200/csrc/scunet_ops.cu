@@ -70,24 +70,30 @@ NormPlan norm_plan(NormGeom g, int vec, int es, bool grad, int sms) {
   NormPlan p{};
   g.cpg = g.c / g.groups;
   g.cols = g.c / vec;
+  g.whole = g.cpg % vec == 0;
   const int bufs = grad ? 2 : 1;
   // ---- small: whole groups whose values fit; at least 64 bytes of a row (two sectors), and
   // some work for a block
   int unit = g.cpg;
   while (unit % vec) unit += g.cpg;
-  const auto fits = [&](long cc) {
-    return cc <= 512L * vec && (double)g.l * cc * es * bufs <= NORM_SMALL_BYTES && cc / g.cpg <= 512;
+  // sums and segments, K, four floats a group; then the values
+  const auto keep = [&](long cc, int threads) {
+    const long segs = cc > threads ? cc : threads;
+    return (2L * vec * threads + 2 * segs + (cc + 1) / 2 * 2 + 4 * (cc / g.cpg) + 3) / 4 * 4;
   };
+  const auto bytes = [&](long cc) { return (double)g.l * cc * es * bufs; };
+  const auto fits = [&](long cc) { return cc <= 512L * vec && 4.0 * keep(cc, 512) + bytes(cc) <= 226 * 1024; };
   if (fits(unit)) {
     long cc = unit;
-    while (cc < g.c && fits(cc + unit) && (cc * es < 64 || (double)g.l * cc * es * bufs < 8192)) cc += unit;
+    while (cc < g.c && fits(cc + unit) && (cc * es < 64 || bytes(cc) < 8192)) cc += unit;
     p.small = true;
-    p.threads = (double)g.l * cc * es * bufs <= 16384 && cc <= 128L * vec ? 128 : 512;
+    p.threads = bytes(cc) <= 16384 && cc <= 128L * vec ? 128 : 512;
     g.tc = (int)(cc / vec);
     g.rp = p.threads / g.tc;
     g.chunks = (int)((g.c + cc - 1) / cc);
     g.splits = 1;
-    p.smem = 4 * ((size_t)(2 * vec + 1) * p.threads + 4 * ((cc / g.cpg + 3) / 4 * 4)) + (size_t)g.l * cc * es * bufs;
+    g.keep = (int)keep(cc, p.threads);
+    p.smem = 4 * (size_t)g.keep + (size_t)g.l * cc * es * bufs;
     p.cpart = grad && g.n > 1 ? (size_t)g.n * g.c : 0;
     p.g = g;
     return p;
@@ -200,11 +206,14 @@ template <typename T, int V, int ACT>
 void norm_two_pass(const NormPlan& p, const NormArgs& a) {
   NormGeom g = p.g;
   const T* x = static_cast<const T*>(a.x);
+  const size_t sum_bytes = 4 * ((size_t)BlockSums<V, NORM_THREADS>::floats(p.g.tc) + (size_t)g.tc * V);  // and K
+  static std::atomic<uint64_t> raised{0};
+  if (allow_smem((const void*)norm_stats_kernel<T, V>, 100 * 1024, raised) != cudaSuccess) return;
   const size_t stat = sizeof(float2) * ((size_t)g.tc * V / g.cpg + 2);
   for (g.first = 0; g.first < g.n; g.first += p.pictures) {
     const long n = g.n - g.first < p.pictures ? g.n - g.first : p.pictures;
     const dim3 grid((unsigned)(n * g.splits), (unsigned)g.chunks);
-    norm_stats_kernel<T, V><<<grid, NORM_THREADS, NORM_THREADS * 4 * (2 * V + 1), a.st>>>(x, a.part, g);
+    norm_stats_kernel<T, V><<<grid, NORM_THREADS, sum_bytes, a.st>>>(x, a.part, g);
     launch_after(norm_apply_kernel<T, V, ACT>, grid, NORM_THREADS, stat, a.st, x, static_cast<T*>(a.y), a.part, a.mean,
                  a.rstd, a.weight, a.bias, g);
   }
@@ -214,11 +223,14 @@ template <typename T, int V, int ACT>
 void norm_two_pass_grad(const NormPlan& p, const NormArgs& a) {
   NormGeom g = p.g;
   const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
+  const size_t sum_bytes = 4 * (size_t)BlockSums<V, NORM_THREADS>::floats(p.g.tc);
+  static std::atomic<uint64_t> raised{0};
+  if (allow_smem((const void*)norm_grad_sums_kernel<T, V, ACT>, 100 * 1024, raised) != cudaSuccess) return;
   const size_t stat = sizeof(float2) * ((size_t)g.tc * V / g.cpg + 2);
   for (g.first = 0; g.first < g.n; g.first += p.pictures) {
     const long n = g.n - g.first < p.pictures ? g.n - g.first : p.pictures;
     const dim3 grid((unsigned)(n * g.splits), (unsigned)g.chunks);
-    norm_grad_sums_kernel<T, V, ACT><<<grid, NORM_THREADS, NORM_THREADS * 8 * V + stat, a.st>>>(
+    norm_grad_sums_kernel<T, V, ACT><<<grid, NORM_THREADS, sum_bytes + stat, a.st>>>(
         dy, x, a.mean, a.rstd, a.weight, a.bias, a.part, a.cpart, g);
     launch_after(norm_grad_apply_kernel<T, V, ACT>, grid, NORM_THREADS, 2 * stat, a.st, dy, x, static_cast<T*>(a.y),
                  a.mean, a.rstd, a.weight, a.bias, a.part, g);
@@ -394,9 +406,6 @@ int scb_group_norm(const void* x, int64_t x_sn, int64_t x_sl, int dtype, int64_t
     if (!(eps >= 0.f)) return refuse(op, "eps must not be negative");
     const int es = elem_size(dtype), sms = sm_count();
     if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
-    const size_t need = norm_work_bytes(n, l, c, groups, sms);
-    if (need && (!work || work_bytes < need || addr(work) % 16))
-      return refuse(op, "the workspace is too small or not 16-byte aligned (scb_group_norm_workspace)");
     if ((mean && addr(mean) % 4) || (rstd && addr(rstd) % 4) || addr(weight) % 4 || addr(bias) % 4)
       return refuse(op, "misaligned float pointer");
     const int vec = norm_vec(es, c, 16, {addr(x), addr(y), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
@@ -406,6 +415,9 @@ int scb_group_norm(const void* x, int64_t x_sn, int64_t x_sl, int dtype, int64_t
     g.n = n; g.l = l; g.c = c; g.groups = groups; g.eps = eps; g.act = act;
     g.x_sn = x_sn; g.x_sl = x_sl; g.y_sn = y_sn; g.y_sl = y_sl;
     const NormPlan p = norm_plan(g, vec, es, false, sms);
+    const size_t need = (p.part + p.cpart) * sizeof(float2);
+    if (need && (!work || work_bytes < need || addr(work) % 16))
+      return refuse(op, "the workspace is too small or not 16-byte aligned (scb_group_norm_workspace)");
     if (n * p.g.splits > kMaxBlocks || p.g.chunks > 65535) return refuse(op, "too many pictures or channels");
     NormArgs a{};
     a.x = x; a.y = y; a.mean = mean; a.rstd = rstd; a.weight = weight; a.bias = bias;
@@ -436,9 +448,6 @@ int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const vo
       return refuse(op, "negative input strides or overlapping output rows");
     const int es = elem_size(dtype), sms = sm_count();
     if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
-    const size_t need = norm_work_bytes(n, l, c, groups, sms);
-    if (need && (!work || work_bytes < need || addr(work) % 16))
-      return refuse(op, "the workspace is too small or not 16-byte aligned (scb_group_norm_workspace)");
     const int vec = norm_vec(es, c, es == 2 ? 8 : 16, {addr(x), addr(dy), addr(dx), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
                                      (uint64_t)(d_sn * es), (uint64_t)(d_sl * es), (uint64_t)(dx_sn * es),
                                      (uint64_t)(dx_sl * es)});
@@ -447,6 +456,9 @@ int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const vo
     g.n = n; g.l = l; g.c = c; g.groups = groups; g.act = act;
     g.x_sn = x_sn; g.x_sl = x_sl; g.y_sn = dx_sn; g.y_sl = dx_sl; g.d_sn = d_sn; g.d_sl = d_sl;
     const NormPlan p = norm_plan(g, vec, es, true, sms);
+    const size_t need = (p.part + p.cpart) * sizeof(float2);
+    if (need && (!work || work_bytes < need || addr(work) % 16))
+      return refuse(op, "the workspace is too small or not 16-byte aligned (scb_group_norm_workspace)");
     if (n * p.g.splits > kMaxBlocks || p.g.chunks > 65535) return refuse(op, "too many pictures or channels");
     NormArgs a{};
     a.dy = dy; a.x = x; a.y = dx; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);

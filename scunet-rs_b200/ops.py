@@ -15,6 +15,7 @@ raise `BackendError`; there is no fallback for tensors that are not on a CUDA de
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -23,23 +24,63 @@ from .backend import (SCB_ACTS, SCB_BF16, SCB_F16, SCB_F32, SCB_I32, SCB_I64, SC
 
 _DTYPES = {torch.float32: SCB_F32, torch.float16: SCB_F16, torch.bfloat16: SCB_BF16}
 _POSITIONS = {torch.int32: SCB_I32, torch.int64: SCB_I64, torch.float32: SCB_F32}
+_lib = None
 
 
 def _fail(msg):
     raise BackendError(msg)
 
 
-def _check(rc, lib):
+def _library():
+    global _lib
+    if _lib is None:
+        _lib = load_library()
+    return _lib
+
+
+# The handle of a device's current stream: torch.cuda.current_stream(index).cuda_stream
+# without the Stream object, which costs 2 us a call.
+_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(t, fn, *args):
+    """fn(*args, stream) on the current stream of t's device; a failure raises its message."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
     if rc != 0:
-        raise BackendError(lib.scb_last_error(None).decode())
+        _fail(_library().scb_last_error(None).decode())
+
+
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(name, device, *sizes):
+    """The workspace of an operator for these sizes on this device."""
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(device):
+        if getattr(_library(), name)(*sizes, ctypes.byref(need)) != 0:
+            _fail(_library().scb_last_error(None).decode())
+    return need.value
+
+
+def _workspace(name, t, *sizes):
+    """(tensor to keep until the call is launched, its address, its bytes)"""
+    need = _work_bytes(name, t.device.index, *sizes)
+    if not need:
+        return None, None, 0
+    work = torch.empty(need, dtype=torch.uint8, device=t.device)
+    return work, work.data_ptr(), need
 
 
 def _dtype(t, what):
     if not t.is_cuda:
         _fail(f"{what} must be on a CUDA device")
-    if t.dtype not in _DTYPES:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
         _fail(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
-    return _DTYPES[t.dtype]
+    return dt
 
 
 def _same(t, like, what):
@@ -59,11 +100,14 @@ def _params(t, c, like, what):
 def _rows(t, what):
     """(pictures, rows, channels, picture stride, row stride) of [n][...][c]; the dimensions
     between collapse to rows of one stride."""
-    if t.dim() < 2:
-        _fail(f"{what} must be [pictures, ..., channels]")
     shape, stride = t.shape, t.stride()
+    dims = len(shape)
+    if dims < 2:
+        _fail(f"{what} must be [pictures, ..., channels]")
     if shape[-1] > 1 and stride[-1] != 1:
         _fail(f"{what}: the channels must be contiguous (channels last)")
+    if dims == 3:
+        return shape[0], shape[1], shape[2], stride[0], stride[1]
     rows, sl = 1, 0
     for size, st in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
         if size == 1:
@@ -76,18 +120,22 @@ def _rows(t, what):
     return shape[0], rows, shape[-1], stride[0], sl
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _workspace(fn, lib, device, *sizes):
-    need = ctypes.c_size_t(0)
-    _check(fn(*sizes, ctypes.byref(need)), lib)
-    return torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+def _out(out, like, what="out"):
+    """`out`, checked, or new contiguous memory of like's shape."""
+    if out is None:
+        return like.new_empty(like.shape)
+    _same(out, like, what)
+    return out
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _act(act):
+    if act not in SCB_ACTS:
+        _fail(f"unknown activation {act!r}")
+    return SCB_ACTS[act]
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act="none", out=None, stats=False):
@@ -98,23 +146,15 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act="none", out=N
     With stats=True also returns mean and 1 / sqrt(var + eps), float32 [n, groups]."""
     dt = _dtype(x, "x")
     n, l, c, sn, sl = _rows(x, "x")
-    if act not in SCB_ACTS:
-        _fail(f"unknown activation {act!r}")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _same(out, x, "out")
-    _, _, _, on, ol = _rows(out, "out")
-    w, b = _params(weight, c, x, "weight"), _params(bias, c, x, "bias")
-    lib = load_library()
-    with torch.cuda.device(x.device):
-        mean = rstd = None
-        if stats:
-            mean, rstd = (torch.empty((n, max(groups, 1)), dtype=torch.float32, device=x.device) for _ in range(2))
-        work = _workspace(lib.scb_group_norm_workspace, lib, x.device, n, l, c, groups)
-        _check(lib.scb_group_norm(x.data_ptr(), sn, sl, dt, n, l, c, groups, w, b, eps, SCB_ACTS[act], out.data_ptr(),
-                                  on, ol, _ptr(mean), _ptr(rstd), _ptr(work), 0 if work is None else work.numel(), _stream(x)), lib)
-    return (out, mean, rstd) if stats else out
+    y = _out(out, x)
+    yn, yl = (l * c, c) if out is None else _rows(y, "out")[3:]
+    mean = rstd = None
+    if stats:
+        mean, rstd = (torch.empty((n, max(groups, 1)), dtype=torch.float32, device=x.device) for _ in range(2))
+    _work, work, size = _workspace("scb_group_norm_workspace", x, n, l, c, groups)
+    _call(x, _library().scb_group_norm, x.data_ptr(), sn, sl, dt, n, l, c, groups, _params(weight, c, x, "weight"),
+          _params(bias, c, x, "bias"), eps, _act(act), y.data_ptr(), yn, yl, _ptr(mean), _ptr(rstd), work, size)
+    return (y, mean, rstd) if stats else y
 
 
 def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, act="none", out=None):
@@ -125,34 +165,28 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, ac
     n, l, c, sn, sl = _rows(x, "x")
     _same(dy, x, "dy")
     _, _, _, dn, dl = _rows(dy, "dy")
-    if act not in SCB_ACTS:
-        _fail(f"unknown activation {act!r}")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _same(out, x, "out")
-    _, _, _, on, ol = _rows(out, "out")
-    w, b = _params(weight, c, x, "weight"), _params(bias, c, x, "bias")
+    dx = _out(out, x)
+    xn, xl = (l * c, c) if out is None else _rows(dx, "out")[3:]
     for t, what in ((mean, "mean"), (rstd, "rstd")):
         if t.dtype != torch.float32 or t.device != x.device or t.shape != (n, groups) or not t.is_contiguous():
             _fail(f"{what} must be contiguous float32 [{n}, {groups}] on {x.device}")
-    lib = load_library()
-    with torch.cuda.device(x.device):
-        dw, db = (torch.empty(c, dtype=torch.float32, device=x.device) for _ in range(2))
-        work = _workspace(lib.scb_group_norm_workspace, lib, x.device, n, l, c, groups)
-        _check(lib.scb_group_norm_backward(dy.data_ptr(), dn, dl, x.data_ptr(), sn, sl, dt, n, l, c, groups,
-                                           mean.data_ptr(), rstd.data_ptr(), w, b, SCB_ACTS[act], out.data_ptr(), on,
-                                           ol, dw.data_ptr(), db.data_ptr(), _ptr(work), 0 if work is None else work.numel(),
-                                           _stream(x)), lib)
-    return out, dw, db
+    dparams = torch.empty((2, c), dtype=torch.float32, device=x.device)
+    dw, db = dparams.unbind(0)
+    _work, work, size = _workspace("scb_group_norm_workspace", x, n, l, c, groups)
+    _call(x, _library().scb_group_norm_backward, dy.data_ptr(), dn, dl, x.data_ptr(), sn, sl, dt, n, l, c, groups,
+          mean.data_ptr(), rstd.data_ptr(), _params(weight, c, x, "weight"), _params(bias, c, x, "bias"), _act(act),
+          dx.data_ptr(), xn, xl, dw.data_ptr(), db.data_ptr(), work, size)
+    return dx, dw, db
 
 
 def _heads(x, out, what):
     if x.dim() != 4:
         _fail(f"{what} must be [pictures, tokens, heads, channels]")
-    if x.shape[3] > 1 and (x.stride(3) != 1 or out.stride(3) != 1):
+    xb, xl, xh, xd = x.stride()
+    yb, yl, yh, yd = out.stride()
+    if x.shape[3] > 1 and (xd != 1 or yd != 1):
         _fail(f"{what}: the channels must be contiguous")
-    return ScbHeads(x.data_ptr(), out.data_ptr(), x.shape[2], *x.stride()[:3], *out.stride()[:3])
+    return ScbHeads(x.data_ptr(), out.data_ptr(), x.shape[2], xb, xl, xh, yb, yl, yh)
 
 
 def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=False, out=None):
@@ -183,20 +217,12 @@ def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=F
     else:
         _fail(f"positions must be [{l}, {axes}] or [{b}, {l}, {axes}], not {tuple(positions.shape)}")
     _params(inv_freq, sum(sections), q, "inv_freq")
-    if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
-               None if k is None else torch.empty(k.shape, dtype=k.dtype, device=q.device))
-    _same(out[0], q, "out[0]")
-    qh, kh = _heads(q, out[0], "q"), None
-    if k is not None:
-        _same(out[1], k, "out[1]")
-        kh = _heads(k, out[1], "k")
-    lib = load_library()
-    with torch.cuda.device(q.device):
-        _check(lib.scb_rotate_axes(qh, kh, dt, b, l, d, positions.data_ptr(), _POSITIONS[positions.dtype], pb, pl, pa,
-                                   inv_freq.data_ptr(), (ctypes.c_int * axes)(*sections), axes,
-                                   SCB_ROT_LAYOUTS[layout], bool(inverse), _stream(q)), lib)
-    return out
+    yq = _out(None if out is None else out[0], q, "out[0]")
+    yk = None if k is None else _out(None if out is None else out[1], k, "out[1]")
+    _call(q, _library().scb_rotate_axes, _heads(q, yq, "q"), None if k is None else _heads(k, yk, "k"), dt, b, l, d,
+          positions.data_ptr(), _POSITIONS[positions.dtype], pb, pl, pa, inv_freq.data_ptr(),
+          (ctypes.c_int * axes)(*sections), axes, SCB_ROT_LAYOUTS[layout], bool(inverse))
+    return yq, yk
 
 
 def attention(q, k, v, *, scale=None, key_mask=None, out=None):
@@ -220,20 +246,17 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
         if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.device != q.device \
                 or key_mask.shape != (b, lk) or (lk > 1 and key_mask.stride(1) != 1):
             _fail(f"key_mask must be bool or uint8 [{b}, {lk}] on {q.device}, its rows contiguous")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _same(out, q, "out")
-        if d > 1 and out.stride(3) != 1:
-            _fail("out: the channels must be contiguous")
-    lib = load_library()
-    with torch.cuda.device(q.device):
-        work = _workspace(lib.scb_attention_workspace, lib, q.device, b, lq, lk, h, hk, d)
-        rows = [ScbRows(t.data_ptr(), *t.stride()[:3]) for t in (q, k, v, out)]
-        _check(lib.scb_attention(*rows, dt, b, lq, lk, h, hk, d, _ptr(key_mask),
-                                 0 if key_mask is None else key_mask.stride(0), d ** -0.5 if scale is None else scale,
-                                 _ptr(work), 0 if work is None else work.numel(), _stream(q)), lib)
-    return out
+    o = _out(out, q)
+    if d > 1 and o.stride(3) != 1:
+        _fail("out: the channels must be contiguous")
+    rows = []
+    for t in (q, k, v, o):
+        sb, sl, sh, _ = t.stride()
+        rows.append(ScbRows(t.data_ptr(), sb, sl, sh))
+    _work, work, size = _workspace("scb_attention_workspace", q, b, lq, lk, h, hk, d)
+    _call(q, _library().scb_attention, *rows, dt, b, lq, lk, h, hk, d, _ptr(key_mask),
+          0 if key_mask is None else key_mask.stride(0), d ** -0.5 if scale is None else scale, work, size)
+    return o
 
 
 def status(stream=None):
@@ -241,8 +264,8 @@ def status(stream=None):
     on a bounded wait since the last call; its outputs are undefined then."""
     stream = stream or torch.cuda.current_stream()
     with torch.cuda.device(stream.device):
-        lib = load_library()
-        _check(lib.scb_op_status(stream.cuda_stream), lib)
+        if _library().scb_op_status(stream.cuda_stream) != 0:
+            _fail(_library().scb_last_error(None).decode())
 
 
 class GroupNormAct(torch.autograd.Function):
@@ -275,5 +298,6 @@ class RotateAxes(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
-        dq, dk = rotate_axes(dq.contiguous(), dk.contiguous(), positions, inv_freq, ctx.sections, layout=ctx.layout, inverse=True)
+        dq, dk = rotate_axes(dq.contiguous(), dk.contiguous(), positions, inv_freq, ctx.sections, layout=ctx.layout,
+                             inverse=True)
         return dq, dk, None, None, None, None
