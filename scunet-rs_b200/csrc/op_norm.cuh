@@ -11,10 +11,10 @@
 //  * norm_small_kernel: a picture's rows of a few whole groups fit in one block's shared
 //    memory; the values are read once, one launch.
 //  * norm_stats_kernel, then norm_apply_kernel (norm_grad_sums_kernel, then
-//    norm_grad_apply_kernel): blocks take row ranges of all pictures and leave one partial
-//    per group; the second launch starts while the first one ends, every block joins its
-//    picture's partials itself, and walks its rows backwards, so that what the first pass
-//    read last is still in L2.
+//    norm_grad_apply_kernel): blocks take rows of all pictures and leave one partial per
+//    group; the second launch starts while the first one ends and every block joins its
+//    picture's partials itself. (Walking the second pass backwards, to meet what the first
+//    read last in L2, measured 3 to 9 % slower than forwards.)
 // A thread keeps its channels (a vector of up to 16 bytes) and steps over rows.
 //
 // Statistics are fp32: a block sums x - K and (x - K)^2 with K the median of the channel's
@@ -29,23 +29,27 @@ namespace scb {
 
 struct NormGeom {
   long n, l;          // pictures, rows of each
-  long first;         // first picture of the launch
   int c, groups, cpg; // channels, groups, channels per group
   int cols;           // vectors of a row
   int tc, rp;         // vectors of a row that one block takes (a chunk), rows it takes at once
   int chunks, slots;  // chunks of a row; groups + chunks - 1 partials of a split: a chunk's
                       // part of a group is slot group + chunk (a group may span chunks)
   int splits;         // row ranges of a picture
+  long cycles;        // l / (rp * splits)
   int whole;          // a vector never spans two groups
   long x_sn, x_sl;    // element strides of pictures and rows
   long y_sn, y_sl;
   long d_sn, d_sl;    // dy
   float eps;
   int act;            // read by the kernels compiled for ACT_ANY
-  int keep;           // small form: where the values start in shared memory, in floats
+  int keep;           // floats of shared memory before the values (small form), the ring (second
+                      // pass) or what lies behind the ring (first pass)
 };
 
 constexpr int NORM_THREADS = 512;  // two blocks an SM: every block reads its picture's partials
+
+// Blocks of the gradient an SM: vectors of 8 take more than the 64 registers that two leave.
+__host__ __device__ constexpr int norm_grad_blocks(int vec) { return vec == 8 ? 1 : 2; }
 
 struct Moments {
   float n, mean, m2;
@@ -90,56 +94,82 @@ __device__ __forceinline__ Pack<T, V> repack(const float* v) {
   return a;
 }
 
-// Activations of V values. SiLU takes one reciprocal for two values (1/a = b / (ab)): the
-// special function unit, at two operations a value, would bound the pass; e^-z is capped at
-// 2^60, where the product stays finite and z sigmoid(z) is 0 to 1e-17.
-template <int ACT, int V>
-__device__ __forceinline__ void sigmoids(const float* z, float* s) {
-#pragma unroll
-  for (int i = 0; i < V; i += 2) {
-    const float a = 1.f + ex2_approx(fminf(z[i] * -1.4426950408889634f, 60.f));
-    if (i + 1 < V) {
-      const float b = 1.f + ex2_approx(fminf(z[i + 1] * -1.4426950408889634f, 60.f));
-      const float r = rcp_approx(a * b);
-      s[i] = b * r;
-      s[i + 1] = a * r;
-    } else {
-      s[i] = rcp_approx(a);
-    }
-  }
+// 1 / (1 + e^-z) of two values: e^-z overflows to inf below z = -88, whose reciprocal is 0.
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+  const float2 t = __fmul2_rn(z, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  const float2 d = __fadd2_rn(make_float2(ex2_approx(t.x), ex2_approx(t.y)), make_float2(1.f, 1.f));
+  return make_float2(rcp_approx(d.x), rcp_approx(d.y));
 }
+
+// The activation, and its slope, of V values; SiLU two at a time (packed arithmetic halves
+// the instructions, which bound these passes before memory does).
 template <int ACT, int V>
 __device__ __forceinline__ void act_all(const NormGeom& g, float* z) {
-  if (ACT == ACT_SILU) {
-    float s[V];
-    sigmoids<ACT, V>(z, s);
-#pragma unroll
-    for (int i = 0; i < V; ++i) z[i] *= s[i];
-  } else if (ACT == ACT_ANY) {
+  if constexpr (ACT == ACT_ANY) {
     if (g.act == ACT_SILU) return act_all<ACT_SILU, V>(g, z);
     if (g.act == ACT_GELU) return act_all<ACT_GELU, V>(g, z);
     if (g.act == ACT_RELU) return act_all<ACT_RELU, V>(g, z);
+  } else if constexpr (ACT == ACT_SILU && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 v = make_float2(z[i], z[i + 1]), r = __fmul2_rn(v, sigmoid2(v));
+      z[i] = r.x;
+      z[i + 1] = r.y;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] = act_fwd<ACT>(z[i]);
   }
 }
-// z -> act'(z)
 template <int ACT, int V>
 __device__ __forceinline__ void slope_all(const NormGeom& g, float* z) {
-  if (ACT == ACT_SILU) {
-    float s[V];
-    sigmoids<ACT, V>(z, s);
-#pragma unroll
-    for (int i = 0; i < V; ++i) z[i] = s[i] * (1.f + z[i] * (1.f - s[i]));
-  } else if (ACT == ACT_ANY) {
+  if constexpr (ACT == ACT_ANY) {
     if (g.act == ACT_SILU) return slope_all<ACT_SILU, V>(g, z);
     if (g.act == ACT_GELU) return slope_all<ACT_GELU, V>(g, z);
     if (g.act == ACT_RELU) return slope_all<ACT_RELU, V>(g, z);
     return slope_all<ACT_NONE, V>(g, z);
+  } else if constexpr (ACT == ACT_SILU && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      // s (1 + z (1 - s)) = s + (z s) (1 - s)
+      const float2 v = make_float2(z[i], z[i + 1]), s = sigmoid2(v);
+      const float2 zs = __fmul2_rn(v, s);
+      const float2 r = __ffma2_rn(make_float2(-s.x, -s.y), zs, __fadd2_rn(s, zs));
+      z[i] = r.x;
+      z[i + 1] = r.y;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) z[i] = act_slope<ACT>(z[i]);
+  }
+}
+
+// r = a b + c of V values; Nb, Nc: 1 where b, c are one value for all
+template <int V, int Nb = V, int Nc = V>
+__device__ __forceinline__ void fma_all(const float* a, const float* b, const float* c, float* r) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const int j = Nb == 1 ? 0 : i, j1 = Nb == 1 ? 0 : i + 1, k = Nc == 1 ? 0 : i, k1 = Nc == 1 ? 0 : i + 1;
+      const float2 t = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[j], b[j1]), make_float2(c[k], c[k1]));
+      r[i] = t.x;
+      r[i + 1] = t.y;
+    }
+  } else {
+    r[0] = fmaf(a[0], b[0], c[0]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_all(const float* a, const float* b, float* r) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 t = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+      r[i] = t.x;
+      r[i + 1] = t.y;
+    }
+  } else {
+    r[0] = a[0] * b[0];
   }
 }
 
@@ -165,23 +195,24 @@ struct Channels {
     }
   }
   __device__ __forceinline__ void z(const float* x, float* out) const {
-#pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = fmaf(x[i], sc[i], sh[i]);
+    fma_all<V>(x, sc, sh, out);
   }
 };
-// xh = x rs + mr of the same channels, for the gradient.
+// xh = x rs + mr of the same channels, for the gradient. Vectors of 8 lie in one group (the
+// gradient takes narrower ones where groups are not multiples of 8 wide), so one value each.
 template <int V>
 struct Hats {
-  float rs[V], mr[V];
+  static constexpr int kN = V == 8 ? 1 : V;
+  float rs[kN], mr[kN];
   __device__ __forceinline__ void load(const NormGeom& g, const float2* stats, int first_group, int c0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < kN; ++i) {
       const float2 st = stats[group_of(g, c0, i) - first_group];
       rs[i] = st.y;
       mr[i] = -st.x * st.y;
     }
   }
-  __device__ __forceinline__ float at(int i, float x) const { return fmaf(x, rs[i], mr[i]); }
+  __device__ __forceinline__ void of(const float* x, float* out) const { fma_all<V, kN, kN>(x, rs, mr, out); }
 };
 
 // A block's sums of two values per channel over its row lanes. Every thread leaves its V
@@ -256,13 +287,13 @@ __device__ __forceinline__ float2 group_moments(const BlockSums<V, T>& s, const 
   return make_float2(mean, warp_sum(m2));
 }
 
-// The channels' K for rows [r0, r1) of a block.
+// The channels' K from `many` rows, `stride` elements apart.
 template <typename T, int V>
-__device__ __forceinline__ void middle_of_rows(const T* src, long stride, long r0, long r1, float* k) {
+__device__ __forceinline__ void middle_of_rows(const T* src, long stride, long many, float* k) {
   Pack<T, V> a, b, c;
-  a.load(src + r0 * stride);
-  b.load(src + (r0 + (r1 - r0) / 2) * stride);
-  c.load(src + (r1 - 1) * stride);
+  a.load(src);
+  b.load(src + many / 2 * stride);
+  c.load(src + (many - 1) * stride);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const float x = to_f32(a.v[i]), y = to_f32(b.v[i]), z = to_f32(c.v[i]);
@@ -270,39 +301,135 @@ __device__ __forceinline__ void middle_of_rows(const T* src, long stride, long r
   }
 }
 
-// s += v - k, q += (v - k)^2
+// s += v - k, q += (v - k)^2; two channels an instruction where there are two
 template <int V>
 __device__ __forceinline__ void add_moments(const float* v, const float* k, float* s, float* q) {
+  if constexpr (V % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float d = v[i] - k[i];
-    s[i] += d;
-    q[i] = fmaf(d, d, q[i]);
+    for (int i = 0; i < V; i += 2) {
+      const float2 d = __fadd2_rn(make_float2(v[i], v[i + 1]), make_float2(-k[i], -k[i + 1]));
+      add2_f32x2(s + i, d.x, d.y);
+      const float2 e = __ffma2_rn(d, d, make_float2(q[i], q[i + 1]));
+      q[i] = e.x;
+      q[i + 1] = e.y;
+    }
+  } else {
+    const float d = v[0] - k[0];
+    s[0] += d;
+    q[0] = fmaf(d, d, q[0]);
   }
 }
 
-// The row range of split s.
-__device__ __forceinline__ void norm_rows(const NormGeom& g, int s, long& r0, long& r1) {
-  r0 = g.l * s / g.splits;
-  r1 = g.l * (s + 1) / g.splits;
+// A thread's vectors of successive rows, copied ahead into its own places of a ring in shared
+// memory (cp.async: no registers wait for them, no barrier since nobody else reads them).
+// Plain loads, two rows a thread in flight, left the pass waiting for memory at 2/3 of its
+// rate. `Tensors` streams of the same rows run together. Vectors under 4 bytes are loaded
+// when they are used.
+template <typename T, int V, int Tensors, int Threads>
+struct RowStream {
+  static constexpr int kBytes = V * (int)sizeof(T), kRows = 2;          // rows of a group
+  static constexpr int kGroups = kBytes * Tensors > 16 ? 2 : 4;         // groups in flight: 64 KB a block at most
+  static constexpr bool kAsync = kBytes >= 4;
+  static constexpr int kSmem = kAsync ? kGroups * kRows * Tensors * Threads * kBytes : 0;
+  unsigned char* mine;
+  const T* src[Tensors];  // of the thread's next row to copy
+  long step[Tensors];
+  long left;              // rows still to copy
+  int put, get;
+  __device__ __forceinline__ void place(long k, int t, unsigned char*& at, int group) {
+    at = mine + ((group * kRows + (int)k) * Tensors + t) * (Threads * kBytes);
+  }
+  __device__ __forceinline__ void fetch() {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (left > 0) {
+#pragma unroll
+        for (int t = 0; t < Tensors; ++t) {
+          unsigned char* at;
+          place(k, t, at, put);
+          if constexpr (kBytes == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at)), "l"(src[t]) : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(at)), "l"(src[t]), "n"(kBytes)
+                         : "memory");
+          src[t] += step[t];
+        }
+        --left;
+      }
+    }
+    cp_async_commit();
+    put = put + 1 == kGroups ? 0 : put + 1;
+  }
+  // `n` rows from `first` on, `step` elements apart
+  __device__ __forceinline__ void start(void* ring, long n) {
+    mine = static_cast<unsigned char*>(ring) + threadIdx.x * kBytes;
+    left = n;
+    put = get = 0;
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int k = 0; k + 1 < kGroups; ++k) fetch();
+    }
+  }
+  // The next group's rows, `n` of them wanted (the rest of `a` is not touched).
+  __device__ __forceinline__ void next(int n, Pack<T, V> (*a)[Tensors]) {
+    if constexpr (kAsync) {
+      fetch();
+      asm volatile("cp.async.wait_group %0;" ::"n"(kGroups - 1) : "memory");
+#pragma unroll
+      for (int k = 0; k < kRows; ++k)
+        if (k < n) {
+#pragma unroll
+          for (int t = 0; t < Tensors; ++t) {
+            unsigned char* at;
+            place(k, t, at, get);
+            a[k][t] = *reinterpret_cast<const Pack<T, V>*>(at);
+          }
+        }
+      get = get + 1 == kGroups ? 0 : get + 1;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k)
+        if (k < n) {
+#pragma unroll
+          for (int t = 0; t < Tensors; ++t) {
+            a[k][t].load(src[t]);
+            src[t] += step[t];
+          }
+        }
+    }
+  }
+};
+
+// Split s of a picture takes rp rows of every rp * splits: all blocks together walk through
+// memory side by side (a range of rows for each block was 10 % slower on maps past L2).
+// How many rows that is.
+__device__ __forceinline__ float norm_rows(const NormGeom& g, int s) {
+  const long rest = g.l - g.cycles * g.rp * g.splits - (long)s * g.rp;
+  return (float)(g.cycles * g.rp + (rest <= 0 ? 0 : rest < g.rp ? rest : g.rp));
 }
 
 // A block's place: picture, split, chunk, its thread's vector and row lane.
 struct NormPlace {
-  long pic, r0, r1;
+  long pic, first, step;  // the thread's first row, from one of its rows to the next
   int split, chunk, col, lane;
   bool on;
   int c0, c1;  // the chunk's channels
   __device__ __forceinline__ NormPlace(const NormGeom& g, int vec) {
-    pic = g.first + blockIdx.x / g.splits;
+    pic = blockIdx.x / g.splits;
     split = (int)(blockIdx.x % g.splits);
     chunk = blockIdx.y;
-    col = chunk * g.tc + threadIdx.x % g.tc;
     lane = threadIdx.x / g.tc;
+    col = chunk * g.tc + threadIdx.x - lane * g.tc;
     on = lane < g.rp && col < g.cols;
-    norm_rows(g, split, r0, r1);
+    first = split * g.rp + lane;
+    step = (long)g.rp * g.splits;
     c0 = chunk * g.tc * vec;
     c1 = min(c0 + g.tc * vec, g.c);
+  }
+  // the thread's rows
+  __device__ __forceinline__ long mine(const NormGeom& g) const {
+    const long most = g.cycles + (first + g.cycles * step < g.l);
+    return on ? most : 0;
   }
 };
 
@@ -321,31 +448,53 @@ norm_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, const __gr
   float k[V], sum[V], sq[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) k[i] = sum[i] = sq[i] = 0.f;
-  float* first = norm_sm + BlockSums<V, NORM_THREADS>::floats(g.tc);  // K of the chunk's channels
-  if (p.on && p.r0 < p.r1) {
+  float* first = norm_sm + g.keep;  // K of the chunk's channels, behind the ring and, later, the sums
+  if (p.on && p.first - p.lane < g.l) {
     const T* src = x + p.pic * g.x_sn + (long)p.col * V;
-    Pack<T, V> a;
-    float v[V];
-    middle_of_rows<T, V>(src, g.x_sl, p.r0, p.r1, k);
-#pragma unroll 4
-    for (long row = p.r0 + p.lane; row < p.r1; row += g.rp) {
-      a.load(src + row * g.x_sl);
-      unpack(a, v);
-      add_moments<V>(v, k, sum, sq);
+    using Stream = RowStream<T, V, 1, NORM_THREADS>;
+    Stream rows;
+    long n = p.mine(g);
+    rows.src[0] = src + p.first * g.x_sl;
+    rows.step[0] = p.step * g.x_sl;
+    rows.start(norm_sm, n);
+    // of the block's rows of lane 0: the same K for every lane
+    const long top = p.first - p.lane, many = g.cycles + (top + g.cycles * p.step < g.l);
+    middle_of_rows<T, V>(src + top * g.x_sl, p.step * g.x_sl, many, k);
+    for (; n > 0; n -= Stream::kRows) {
+      Pack<T, V> a[Stream::kRows][1];
+      const int now = n < Stream::kRows ? (int)n : Stream::kRows;
+      rows.next(now, a);
+#pragma unroll
+      for (int r = 0; r < Stream::kRows; ++r) {
+        if (r >= now) break;
+        float v[V];
+        unpack(a[r][0], v);
+        add_moments<V>(v, k, sum, sq);
+      }
     }
   }
   if (p.lane == 0) {
 #pragma unroll
     for (int i = 0; i < V; ++i) first[threadIdx.x * V + i] = k[i];
   }
+  __syncthreads();  // the sums lie over the ring
   BlockSums<V, NORM_THREADS> sums;
   sums.add(norm_sm, g, sum, sq, p.lane);
   float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
   for (int grp = p.c0 / g.cpg + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
     const float2 m = group_moments(sums, first, max(grp * g.cpg, p.c0) - p.c0, min((grp + 1) * g.cpg, p.c1) - p.c0,
-                                   (float)(p.r1 - p.r0));
+                                   norm_rows(g, p.split));
     if ((threadIdx.x & 31) == 0) out[grp] = m;
   }
+}
+
+// Partials s0, s0 + 32, ... of a picture's slot, all on their way at once.
+constexpr int kJoinBatch = 10;
+__device__ __forceinline__ void load_partials(const NormGeom& g, const float2* part, long pic, int slot, int s0,
+                                              float2* v) {
+#pragma unroll
+  for (int b = 0; b < kJoinBatch; ++b)
+    if (s0 + 32 * b < g.splits) v[b] = __ldcg(part + (pic * g.splits + s0 + 32 * b) * g.slots + slot);
 }
 
 // A picture's group, joined over splits (and chunks) by one warp: (mean, rstd).
@@ -353,13 +502,14 @@ __device__ __forceinline__ float2 norm_join(const NormGeom& g, const float2* par
   const int per = g.tc * vec;  // channels of a chunk
   const int k0 = grp * g.cpg / per, k1 = ((grp + 1) * g.cpg - 1) / per;
   Moments m{0.f, 0.f, 0.f};
-  for (int s = threadIdx.x & 31; s < g.splits; s += 32) {
-    long r0, r1;
-    norm_rows(g, s, r0, r1);
-    for (int k = k0; k <= k1; ++k) {
-      const int width = min((grp + 1) * g.cpg, (k + 1) * per) - max(grp * g.cpg, k * per);
-      const float2 v = __ldcg(part + (pic * g.splits + s) * g.slots + grp + k);
-      m = join(m, Moments{(float)(r1 - r0) * (float)width, v.x, v.y});
+  for (int k = k0; k <= k1; ++k) {
+    const float width = (float)(min((grp + 1) * g.cpg, (k + 1) * per) - max(grp * g.cpg, k * per));
+    for (int s0 = threadIdx.x & 31; s0 < g.splits; s0 += 32 * kJoinBatch) {
+      float2 v[kJoinBatch];
+      load_partials(g, part, pic, grp + k, s0, v);
+#pragma unroll
+      for (int b = 0; b < kJoinBatch; ++b)
+        if (s0 + 32 * b < g.splits) m = join(m, Moments{norm_rows(g, s0 + 32 * b) * width, v[b].x, v[b].y});
     }
   }
   m = warp_join(m);
@@ -375,6 +525,14 @@ norm_apply_kernel(const T* x, T* y, const float2* __restrict__ part,
   extern __shared__ __align__(16) float2 norm_stat[];  // of the chunk's groups
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg;
+  // x does not come from the pass before: its first rows are on their way while the partials
+  // are waited for and joined
+  using Stream = RowStream<T, V, 1, NORM_THREADS>;
+  Stream rows;
+  long n = p.mine(g);
+  rows.src[0] = x + p.pic * g.x_sn + p.first * g.x_sl + (long)p.col * V;
+  rows.step[0] = p.step * g.x_sl;
+  rows.start(reinterpret_cast<float*>(norm_stat) + g.keep, n);
   wait_for_previous();
   for (int grp = g0 + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
     const float2 s = norm_join(g, part, p.pic, grp, V);
@@ -387,27 +545,23 @@ norm_apply_kernel(const T* x, T* y, const float2* __restrict__ part,
     }
   }
   __syncthreads();
-  if (!p.on || p.r0 + p.lane >= p.r1) return;
+  if (!n) return;
   Channels<V> ch;
   ch.load(g, norm_stat, g0, p.col * V, weight, bias);
-  const T* src = x + p.pic * g.x_sn + (long)p.col * V;
-  T* dst = y + p.pic * g.y_sn + (long)p.col * V;
-  // batches of loads before their stores: y may be x, so the compiler must not reorder them
-  constexpr int kBatch = sizeof(Pack<T, V>) == 16 ? 2 : 4;
-  const long steps = (p.r1 - p.r0 - p.lane - 1) / g.rp;
-  for (long row = p.r0 + p.lane + steps * g.rp; row >= p.r0; row -= kBatch * g.rp) {
-    Pack<T, V> a[kBatch];
+  T* dst = y + p.pic * g.y_sn + p.first * g.y_sl + (long)p.col * V;
+  for (; n > 0; n -= Stream::kRows) {
+    Pack<T, V> a[Stream::kRows][1];
+    const int now = n < Stream::kRows ? (int)n : Stream::kRows;
+    rows.next(now, a);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-      if (row - b * g.rp >= p.r0) a[b].load(src + (row - b * g.rp) * g.x_sl);
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (row - b * g.rp < p.r0) break;
+    for (int r = 0; r < Stream::kRows; ++r) {
+      if (r >= now) break;
       float v[V];
-      unpack(a[b], v);
+      unpack(a[r][0], v);
       ch.z(v, v);
       act_all<ACT, V>(g, v);
-      repack<T, V>(v).store(dst + (row - b * g.rp) * g.y_sl);
+      repack<T, V>(v).store(dst);
+      dst += p.step * g.y_sl;
     }
   }
 }
@@ -418,8 +572,7 @@ __device__ __forceinline__ void grad_z(const NormGeom& g, const Channels<V>& ch,
                                        float* gz) {
   ch.z(x, gz);
   slope_all<ACT, V>(g, gz);
-#pragma unroll
-  for (int i = 0; i < V; ++i) gz[i] *= dy[i];
+  mul_all<V>(gz, dy, gz);
 }
 
 // (mean, rstd) of the chunk's groups into shared memory.
@@ -436,26 +589,29 @@ __device__ __forceinline__ void add_grad(const NormGeom& g, const Channels<V>& c
   unpack(a, v);
   unpack(e, d);
   grad_z<ACT, V>(g, ch, v, d, gz);
+  hat.of(v, v);
+  if constexpr (V % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    sa[i] += gz[i];
-    sb[i] = fmaf(gz[i], hat.at(i, v[i]), sb[i]);
+    for (int i = 0; i < V; i += 2) add2_f32x2(sa + i, gz[i], gz[i + 1]);
+  } else {
+    sa[0] += gz[0];
   }
+  fma_all<V>(gz, v, sb, sb);
 }
 
 // First pass of the gradient: per (picture, split) the channels' sums of gz and gz xh for dw
 // and db, and the parts of the groups' sums of h and h xh.
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS, 2)
+__global__ void __launch_bounds__(NORM_THREADS, norm_grad_blocks(V))
 norm_grad_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const float* __restrict__ mean,
                       const float* __restrict__ rstd, const float* __restrict__ weight,
                       const float* __restrict__ bias, float2* __restrict__ part, float2* __restrict__ cpart,
                       const __grid_constant__ NormGeom g) {
-  extern __shared__ __align__(16) float norm_sm[];  // the block's sums, then the chunk's groups' statistics
+  extern __shared__ __align__(16) float norm_sm[];  // the ring, then the block's sums; the groups' statistics
   let_next_start();
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg;
-  float2* stats = reinterpret_cast<float2*>(norm_sm + BlockSums<V, NORM_THREADS>::floats(g.tc));
+  float2* stats = reinterpret_cast<float2*>(norm_sm + g.keep);
   grad_stats(g, stats, g0, p.c1, mean, rstd, p.pic);
   __syncthreads();
   float sa[V], sb[V];
@@ -466,16 +622,26 @@ norm_grad_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const f
     Hats<V> hat;
     ch.load(g, stats, g0, p.col * V, weight, bias);
     hat.load(g, stats, g0, p.col * V);
-    const T* src = x + p.pic * g.x_sn + (long)p.col * V;
-    const T* del = dy + p.pic * g.d_sn + (long)p.col * V;
-#pragma unroll 4
-    for (long row = p.r0 + p.lane; row < p.r1; row += g.rp) {
-      Pack<T, V> a, e;
-      a.load(src + row * g.x_sl);
-      e.load(del + row * g.d_sl);
-      add_grad<T, V, ACT>(g, ch, hat, a, e, sa, sb);
+    using Stream = RowStream<T, V, 2, NORM_THREADS>;
+    Stream rows;
+    long n = p.mine(g);
+    rows.src[0] = x + p.pic * g.x_sn + p.first * g.x_sl + (long)p.col * V;
+    rows.src[1] = dy + p.pic * g.d_sn + p.first * g.d_sl + (long)p.col * V;
+    rows.step[0] = p.step * g.x_sl;
+    rows.step[1] = p.step * g.d_sl;
+    rows.start(norm_sm, n);
+    for (; n > 0; n -= Stream::kRows) {
+      Pack<T, V> a[Stream::kRows][2];
+      const int now = n < Stream::kRows ? (int)n : Stream::kRows;
+      rows.next(now, a);
+#pragma unroll
+      for (int r = 0; r < Stream::kRows; ++r) {
+        if (r >= now) break;
+        add_grad<T, V, ACT>(g, ch, hat, a[r][0], a[r][1], sa, sb);
+      }
     }
   }
+  __syncthreads();  // the sums lie over the ring
   BlockSums<V, NORM_THREADS> sums;
   sums.add(norm_sm, g, sa, sb, p.lane);
   float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
@@ -497,8 +663,14 @@ norm_grad_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const f
 __device__ __forceinline__ float2 norm_grad_join(const NormGeom& g, const float2* part, long pic, int grp, int vec) {
   const int per = g.tc * vec, k0 = grp * g.cpg / per, k1 = ((grp + 1) * g.cpg - 1) / per;
   float2 m = make_float2(0.f, 0.f);
-  for (int s = threadIdx.x & 31; s < g.splits; s += 32)
-    for (int k = k0; k <= k1; ++k) m = join(m, __ldcg(part + (pic * g.splits + s) * g.slots + grp + k));
+  for (int k = k0; k <= k1; ++k)
+    for (int s0 = threadIdx.x & 31; s0 < g.splits; s0 += 32 * kJoinBatch) {
+      float2 v[kJoinBatch];
+      load_partials(g, part, pic, grp + k, s0, v);
+#pragma unroll
+      for (int b = 0; b < kJoinBatch; ++b)
+        if (s0 + 32 * b < g.splits) m = join(m, v[b]);
+    }
   m = warp_join(m);
   const float inv = 1.f / ((float)g.l * (float)g.cpg);
   return make_float2(m.x * inv, m.y * inv);
@@ -507,14 +679,15 @@ __device__ __forceinline__ float2 norm_grad_join(const NormGeom& g, const float2
 // dx = gz sc - rs E[h] - xh rs E[h xh] of one vector (sc = rs w).
 template <int V>
 struct GradMeans {
-  float m1[V], m2[V];  // rs E[h], rs E[h xh]
+  static constexpr int kN = Hats<V>::kN;
+  float m1[kN], m2[kN];  // - rs E[h], - rs E[h xh]
   __device__ __forceinline__ void load(const NormGeom& g, const Hats<V>& hat, const float2* means, int first_group,
                                        int c0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
+    for (int i = 0; i < kN; ++i) {
       const float2 m = means[group_of(g, c0, i) - first_group];
-      m1[i] = hat.rs[i] * m.x;
-      m2[i] = hat.rs[i] * m.y;
+      m1[i] = -hat.rs[i] * m.x;
+      m2[i] = -hat.rs[i] * m.y;
     }
   }
 };
@@ -525,13 +698,14 @@ __device__ __forceinline__ Pack<T, V> grad_x(const NormGeom& g, const Channels<V
   unpack(a, v);
   unpack(e, d);
   grad_z<ACT, V>(g, ch, v, d, gz);
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = fmaf(gz[i], ch.sc[i], -m.m1[i]) - hat.at(i, v[i]) * m.m2[i];
+  hat.of(v, v);
+  fma_all<V, V, Hats<V>::kN>(gz, ch.sc, m.m1, gz);
+  fma_all<V, Hats<V>::kN, V>(v, m.m2, gz, v);
   return repack<T, V>(v);
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(NORM_THREADS, 2)
+__global__ void __launch_bounds__(NORM_THREADS, norm_grad_blocks(V))
 norm_grad_apply_kernel(const T* dy, const T* x, T* dx,
                        const float* __restrict__ mean, const float* __restrict__ rstd,
                        const float* __restrict__ weight, const float* __restrict__ bias,
@@ -539,6 +713,14 @@ norm_grad_apply_kernel(const T* dy, const T* x, T* dx,
   extern __shared__ __align__(16) float2 norm_stat[];  // (mean, rstd), then (E[h], E[h xh]) of the chunk's groups
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg, ng = (p.c1 - 1) / g.cpg - g0 + 1;
+  using Stream = RowStream<T, V, 2, NORM_THREADS>;
+  Stream rows;
+  long n = p.mine(g);
+  rows.src[0] = x + p.pic * g.x_sn + p.first * g.x_sl + (long)p.col * V;
+  rows.src[1] = dy + p.pic * g.d_sn + p.first * g.d_sl + (long)p.col * V;
+  rows.step[0] = p.step * g.x_sl;
+  rows.step[1] = p.step * g.d_sl;
+  rows.start(reinterpret_cast<float*>(norm_stat) + g.keep, n);
   grad_stats(g, norm_stat, g0, p.c1, mean, rstd, p.pic);
   wait_for_previous();
   for (int grp = g0 + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
@@ -546,49 +728,46 @@ norm_grad_apply_kernel(const T* dy, const T* x, T* dx,
     if ((threadIdx.x & 31) == 0) norm_stat[ng + grp - g0] = m;
   }
   __syncthreads();
-  if (!p.on || p.r0 + p.lane >= p.r1) return;
+  if (!n) return;
   Channels<V> ch;
   ch.load(g, norm_stat, g0, p.col * V, weight, bias);
   Hats<V> hat;
   GradMeans<V> m;
   hat.load(g, norm_stat, g0, p.col * V);
   m.load(g, hat, norm_stat + ng, g0, p.col * V);
-  const T* src = x + p.pic * g.x_sn + (long)p.col * V;
-  const T* del = dy + p.pic * g.d_sn + (long)p.col * V;
-  T* dst = dx + p.pic * g.y_sn + (long)p.col * V;
-  const long steps = (p.r1 - p.r0 - p.lane - 1) / g.rp;
-  constexpr int kBatch = 2;
-  for (long row = p.r0 + p.lane + steps * g.rp; row >= p.r0; row -= kBatch * g.rp) {
-    Pack<T, V> a[kBatch], e[kBatch];
+  T* dst = dx + p.pic * g.y_sn + p.first * g.y_sl + (long)p.col * V;
+  for (; n > 0; n -= Stream::kRows) {
+    Pack<T, V> a[Stream::kRows][2];
+    const int now = n < Stream::kRows ? (int)n : Stream::kRows;
+    rows.next(now, a);
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (row - k * g.rp >= p.r0) {
-        a[k].load(src + (row - k * g.rp) * g.x_sl);
-        e[k].load(del + (row - k * g.rp) * g.d_sl);
-      }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (row - k * g.rp >= p.r0)
-        grad_x<T, V, ACT>(g, ch, hat, m, a[k], e[k]).store(dst + (row - k * g.rp) * g.y_sl);
+    for (int r = 0; r < Stream::kRows; ++r) {
+      if (r >= now) break;
+      grad_x<T, V, ACT>(g, ch, hat, m, a[r][0], a[r][1]).store(dst);
+      dst += p.step * g.y_sl;
+    }
   }
 }
 
-// dw and db: one warp a channel joins `parts` partials (pictures x splits).
-__global__ void __launch_bounds__(256) norm_grad_params_kernel(const float2* __restrict__ cpart, long parts,
-                                                                        int c, float* __restrict__ dweight,
-                                                                        float* __restrict__ dbias) {
-  // 32 neighbouring channels a block, eight threads each
-  __shared__ float2 sums[8][33];
+// dw and db from `parts` partials (pictures x splits): 32 neighbouring channels a block, 32
+// threads each.
+__global__ void __launch_bounds__(1024) norm_grad_params_kernel(const float2* __restrict__ cpart, long parts, int c,
+                                                                float* __restrict__ dweight,
+                                                                float* __restrict__ dbias) {
+  __shared__ float2 sums[32][33];
   const int ch = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
   float2 m = make_float2(0.f, 0.f);
-  if (ch < c)
-    for (long k = lane; k < parts; k += 8) m = join(m, cpart[k * c + ch]);
-  sums[lane][threadIdx.x & 31] = m;
+  if (ch < c) {
+#pragma unroll 4
+    for (long k = lane; k < parts; k += 32) m = join(m, cpart[k * c + ch]);
+  }
+  sums[threadIdx.x & 31][lane] = m;
   __syncthreads();
-  if (lane == 0 && ch < c) {
-    for (int k = 1; k < 8; ++k) m = join(m, sums[k][threadIdx.x]);
-    if (dbias) dbias[ch] = m.x;
-    if (dweight) dweight[ch] = m.y;
+  m = warp_join(sums[lane][threadIdx.x & 31]);
+  const int mine = blockIdx.x * 32 + lane;
+  if ((threadIdx.x & 31) == 0 && mine < c) {
+    if (dbias) dbias[mine] = m.x;
+    if (dweight) dweight[mine] = m.y;
   }
 }
 
@@ -619,7 +798,7 @@ norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
     if (p.on && g.l > 0) {
       Pack<T, V> a;
       float v[V];
-      middle_of_rows<T, V>(src, g.x_sl, 0, g.l, k);
+      middle_of_rows<T, V>(src, g.x_sl, g.l, k);
 #pragma unroll 4
       for (long row = p.lane; row < g.l; row += g.rp) {
         a.load(src + row * g.x_sl);
