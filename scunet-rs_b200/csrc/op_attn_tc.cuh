@@ -6,7 +6,7 @@
 // tile), or 128 rows when there are no more: then both tiles hold the same rows and take
 // the even and the odd key tiles (`twin`), which keeps two score tiles in flight.
 //
-// Work: all units' key tiles in one line, cut into equal ranges, one per CTA. A CTA walks
+// Work: all units' key tiles in one line, cut into equal ranges, one per CTA (at_start). A CTA walks
 // the units its range touches. A unit that lies in one range is written to the output at
 // once; of a unit that is cut, every piece goes to the workspace as float32 sums with its
 // maximum and total, and attn_join_kernel adds them in order (no atomics).
@@ -44,6 +44,8 @@ struct AttnTcArgs {
   long rows;          // Lq R
   int twin;           // both tiles on the same rows
   int unit_rows;      // 256, or 128 with twin
+  int cuts;           // pieces of a twin unit
+  int turns;          // twin: the tiles' exponentials take turns
   long row_units;     // units of one (picture, key head)
   long units, tiles;  // all units; key tiles of each
   long total;         // units * tiles
@@ -54,7 +56,20 @@ struct AttnTcArgs {
   int q_wide, o_wide; // 16-byte accesses to Q and the output allowed
 };
 
+// Tiles [at_start(cta), at_start(cta + 1)) of the line. Twin units are cut into `cuts` equal
+// pieces instead, one a CTA, pieces of one place next to each other in the grid: all heads
+// then walk the same keys at the same time, and a token's heads lie in the same DRAM page.
 __device__ __forceinline__ long at_start(const AttnTcArgs& g, long cta, long grid) { return cta * g.total / grid; }
+__device__ __forceinline__ void at_range(const AttnTcArgs& g, long cta, long grid, long& x0, long& x1) {
+  if (g.twin) {
+    const long cut = cta / g.units, unit = cta - cut * g.units;
+    x0 = unit * g.tiles + g.tiles * cut / g.cuts;
+    x1 = unit * g.tiles + g.tiles * (cut + 1) / g.cuts;
+  } else {
+    x0 = at_start(g, cta, grid);
+    x1 = at_start(g, cta + 1, grid);
+  }
+}
 // The CTA whose range holds tile x.
 __device__ __forceinline__ long at_owner(const AttnTcArgs& g, long x, long grid) { return ((x + 1) * grid - 1) / g.total; }
 
@@ -139,18 +154,40 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// A bounded wait that gives up at once when another wait of the CTA has given up.
-__device__ __forceinline__ void at_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+// The ring place of a K or V tile, and how often the place was filled before. The tiles of
+// Twin have a half of the ring each: a wait tells a filling only from the one before it, and
+// in a shared ring a tile could be two fillings ahead of loads that only the other waits for.
+template <bool Twin, int Slots>
+struct AtPlace {
+  uint32_t slot, turn;
+  __device__ __forceinline__ explicit AtPlace(uint32_t seq) {
+    if (Twin) {
+      constexpr uint32_t kHalf = Slots / 2;
+      const uint32_t own = (seq >> 2) * 2 + (seq & 1);  // seq: K V of tile 0, K V of tile 1, ...
+      slot = (seq >> 1 & 1) * kHalf + own % kHalf;
+      turn = own / kHalf;
+    } else {
+      slot = seq % Slots;
+      turn = seq / Slots;
+    }
+  }
+};
+
+// A bounded wait that gives up at once when another wait of the CTA has given up. The error
+// word tells the place of the first one that did.
+enum : unsigned { AT_EMPTY = 0x100, AT_FULL = 0x200, AT_Q = 0x300, AT_S = 0x400, AT_FREE = 0x500, AT_P = 0x600, AT_O = 0x700 };
+__device__ __forceinline__ void at_wait(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned place) {
   if (mbar_try_wait(bar, parity)) return;
   if (*dead) return;
-  if (!mbar_wait(bar, parity, SCB_ERR_WAIT_ATTN)) *dead = 1;
+  if (!mbar_wait(bar, parity, SCB_ERR_WAIT_ATTN | place)) *dead = 1;
 }
 
-template <typename T, int Boxes>
+template <typename T, int Boxes, bool Twin>
 __global__ void __launch_bounds__(AT_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                const __grid_constant__ AttnTcArgs g) {
   using L = AtLayout<Boxes>;
+  using Place = AtPlace<Twin, L::kSlots>;
   extern __shared__ __align__(1024) uint8_t sm[];  // the swizzled tiles' alignment
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::kBars);
   uint64_t* empty = full + L::kSlots;
@@ -166,7 +203,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   if (tid == 0) {
     for (int i = 0; i < L::kSlots; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, g.twin ? 1 : 2);  // the tiles that read the slot
+      mbar_init(empty + i, Twin ? 1 : 2);  // the tiles that read the slot
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(q_ready + t, 256);
@@ -184,7 +221,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const long x0 = at_start(g, blockIdx.x, gridDim.x), x1 = at_start(g, blockIdx.x + 1, gridDim.x);
+  long x0, x1;
+  at_range(g, blockIdx.x, gridDim.x, x0, x1);
   const int d = g.a.d, ksteps = (d + 15) / 16;
 
   // 640 x 96 = 61440 registers at launch, 512 x 104 + 128 x 64 = 61440 after the split
@@ -199,21 +237,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         const int b = (int)(bh / g.a.hk), h = (int)(bh - (long)b * g.a.hk);
         for (long j = j0; j < j0 + n; ++j)
           for (int w = 0; w < 2; ++w, ++seq) {  // K, V
-            const uint32_t slot = seq % L::kSlots, turn = seq / L::kSlots;
-            if (turn) at_wait(empty + slot, (turn - 1) & 1, dead);
+            const Place at(seq);
+            if (at.turn) at_wait(empty + at.slot, (at.turn - 1) & 1, dead, AT_EMPTY);
             if (*dead) break;
-            mbar_arrive_expect_tx(full + slot, L::kTile);
+            mbar_arrive_expect_tx(full + at.slot, L::kTile);
             for (int c = 0; c < Boxes; ++c)
-              tma_load_4d(sm + L::kRing + slot * L::kTile + c * AT_BOX, w ? &tv : &tk, full + slot, 64 * c,
+              tma_load_4d(sm + L::kRing + at.slot * L::kTile + c * AT_BOX, w ? &tv : &tk, full + at.slot, 64 * c,
                           (int)(j * AT_KEYS), (g.kv_h >> w & 1) * h, (g.kv_b >> w & 1) * b);
           }
         x += n;
       }
       // after a wait gave up, loads may still be on their way: none may outlive the CTA
       if (*dead)
-        for (uint32_t back = 1; back <= L::kSlots && back <= seq; ++back) {
-          const uint32_t s = seq - back;
-          mbar_wait(full + s % L::kSlots, (s / L::kSlots) & 1, SCB_ERR_WAIT_ATTN);
+        for (uint32_t back = 1; back <= 2 * L::kSlots && back <= seq; ++back) {
+          // (a place that was filled again since passes at once)
+          const Place at(seq - back);
+          mbar_wait(full + at.slot, at.turn & 1, SCB_ERR_WAIT_ATTN);
         }
     } else if (warp < 18 && elect_one()) {
       // ---- matrix products of tile t
@@ -226,50 +265,50 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       const uint64_t dk = make_sdesc(sb + L::kRing, 128, SW_128B);
       const uint64_t dv = make_sdesc_lbo_sbo(sb + L::kRing, AT_BOX, 1024, SW_128B);
       const uint32_t ts = tmem + 128 * t, tp = tmem + L::kP + L::kPStep * t, to = tmem + L::kO + L::kOStep * t;
-      const uint32_t step = g.twin ? 4 : 2;  // ring places from one K to the tile's next
+      const uint32_t step = Twin ? 4 : 2;  // ring places from one K to the tile's next
       uint32_t cnt = 0, segs = 0, base = 0;
       const auto scores = [&](uint32_t seq) {
-        const uint32_t slot = seq % L::kSlots;
-        at_wait(full + slot, (seq / L::kSlots) & 1, dead);
+        const Place at(seq);
+        at_wait(full + at.slot, at.turn & 1, dead, AT_FULL);
         tc_fence_after();
-        const uint64_t k = dk + slot * (uint32_t)(L::kTile >> 4);
+        const uint64_t k = dk + at.slot * (uint32_t)(L::kTile >> 4);
 #pragma unroll
         for (int s = 0; s < 4 * Boxes; ++s) {
           const uint32_t o = ((s >> 2) * AT_BOX + (s & 3) * 32) >> 4;
           if (s < ksteps) umma_f16(ts, dq + o, k + o, id_s, s > 0);
         }
         umma_commit(s_full + t);
-        umma_commit(empty + slot);
+        umma_commit(empty + at.slot);
       };
       for (long x = x0; x < x1;) {
         const long unit = x / g.tiles, j0 = x - unit * g.tiles;
         const uint32_t n = (uint32_t)min(x1 - x, g.tiles - j0);
-        const uint32_t nt = g.twin ? (n + 1 - t) / 2 : n;
-        uint32_t seq = 2 * (base + (g.twin ? t : 0));  // of K; V is the next
+        const uint32_t nt = Twin ? (n + 1 - t) / 2 : n;
+        uint32_t seq = 2 * (base + (Twin ? t : 0));  // of K; V is the next
         if (nt) {
-          at_wait(q_ready + t, segs++ & 1, dead);
+          at_wait(q_ready + t, segs++ & 1, dead, AT_Q);
           tc_fence_after();
           scores(seq);
         }
         for (uint32_t i = 0; i < nt && !*dead; ++i, ++cnt, seq += step) {
           if (L::kOwnP && i + 1 < nt) {  // the next scores, as soon as S_t is in registers
-            at_wait(s_free + t, cnt & 1, dead);
+            at_wait(s_free + t, cnt & 1, dead, AT_FREE);
             scores(seq + step);
           }
-          const uint32_t slot = (seq + 1) % L::kSlots;
-          at_wait(full + slot, ((seq + 1) / L::kSlots) & 1, dead);
-          const uint64_t v = dv + slot * (uint32_t)(L::kTile >> 4);
-          at_wait(p_ready + t, cnt & 1, dead);
+          const Place at(seq + 1);
+          at_wait(full + at.slot, at.turn & 1, dead, AT_FULL);
+          const uint64_t v = dv + at.slot * (uint32_t)(L::kTile >> 4);
+          at_wait(p_ready + t, cnt & 1, dead, AT_P);
           tc_fence_after();
 #pragma unroll
           for (int s = 0; s < AT_KEYS / 16; ++s)
             umma_f16_ts(to, tp + 8 * s, v + (uint32_t)(2048 * s >> 4), id_o, i > 0 || s > 0);
           umma_commit(o_done + t);
-          umma_commit(empty + slot);
+          umma_commit(empty + at.slot);
           if (!L::kOwnP && i + 1 < nt) {
             // S_t overwrites P_t, so P_t V must have read it; the other tile's softmax runs
             // meanwhile
-            at_wait(o_done + t, cnt & 1, dead);
+            at_wait(o_done + t, cnt & 1, dead, AT_O);
             scores(seq + step);
           }
         }
@@ -294,17 +333,23 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const float c = g.a.scale_log2, stale = fminf(AT_STALE / c, 1e30f);
     const int last = (int)(g.tiles - 1), tail = (int)(g.a.lk - (long)last * AT_KEYS) - 64 * half;  // of the last tile, past this half's first key
     uint32_t cnt = 0, base = 0;
-    if (t == 1) at_turn_give(t);
+    if ((!Twin || g.turns) && t == 1) at_turn_give(t);
     for (long x = x0; x < x1;) {
       const long unit = x / g.tiles, j0 = x - unit * g.tiles, n = min(x1 - x, g.tiles - j0);
       const long bh = unit / g.row_units;
       const int b = (int)(bh / g.a.hk), hk = (int)(bh - (long)b * g.a.hk);
-      const long r = (unit - bh * g.row_units) * g.unit_rows + (g.twin ? 0 : 128 * t) + row;
-      const int step = g.twin ? 2 : 1, jt = (int)j0 + (g.twin ? t : 0), jn = (int)(j0 + n);
+      // Twin: tile 1 holds the rows turned by 64, so that few rows are on another scheduler of
+      // the SM than tile 0's
+      const int unit_row = Twin ? (row + 64 * t) & 127 : 128 * t + row;
+      const long r = (unit - bh * g.row_units) * g.unit_rows + unit_row;
+      const int step = Twin ? 2 : 1, jt = (int)j0 + (Twin ? t : 0), jn = (int)(j0 + n);
       const bool any = jt < jn;
       // row rr of this warp's 32 (or -1 past the last): its query and head
       const int warp_row = (warp & 3) * 32;
       const long r0 = r - lane;
+      // a warp with no row left only keeps the others company (with 256 rows of a unit that is
+      // rare, and looking costs 10 %)
+      const bool live = !Twin || r0 < g.rows;
       const auto locate = [&](int rr, int64_t sb, int64_t sl, int64_t sh) -> long {
         const long x = r0 + rr;
         if (x >= g.rows) return -1;
@@ -368,10 +413,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             seen[i] = k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u;
           }
         }
-        at_wait(s_full + t, cnt & 1, dead);
+        at_wait(s_full + t, cnt & 1, dead, AT_S);
         tc_fence_after();
         float s[64];
-        {
+        if (live) {
           uint32_t u[64];
 #pragma unroll
           for (int i = 0; i < 4; ++i) tmem_ld16_issue(ts + 16 * i, u + 16 * i);
@@ -388,23 +433,25 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
         if (part) {
           asm volatile("");  // keeps this a branch: 64 selects would cost every tile
+          if (live) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) s[i] = seen[i >> 5] >> (i & 31) & 1 ? s[i] : -INFINITY;
+            for (int i = 0; i < 64; ++i) s[i] = seen[i >> 5] >> (i & 31) & 1 ? s[i] : -INFINITY;
+          }
           if (mask) {
             // hidden values may be NaN or infinite, and 0 times those is NaN: clear this
             // half's hidden rows of V, 64 threads each half of a row's chunks or boxes
-            const uint32_t seq = 2 * (base + (uint32_t)(j - (int)j0)) + 1, slot = seq % L::kSlots;
-            at_wait(full + slot, (seq / L::kSlots) & 1, dead);
+            const Place at(2 * (base + (uint32_t)(j - (int)j0)) + 1);
+            at_wait(full + at.slot, at.turn & 1, dead, AT_FULL);
             if (!((row & 32 ? seen[1] : seen[0]) >> (row & 31) & 1)) {
-              uint4* v = reinterpret_cast<uint4*>(sm + L::kRing + slot * L::kTile + (64 * half + (row & 63)) * 128 +
+              uint4* v = reinterpret_cast<uint4*>(sm + L::kRing + at.slot * L::kTile + (64 * half + (row & 63)) * 128 +
                                                   (row >> 6) * (Boxes == 2 ? AT_BOX : 64));
               for (int k = 0; k < 4 * Boxes; ++k) v[k] = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
           }
         }
-        float top = row_max<64>(s);
-        if (cnt > first) at_wait(o_done + t, (cnt - 1) & 1, dead);  // O_t is complete, P_t read
+        float top = live ? row_max<64>(s) : -INFINITY;
+        if (cnt > first) at_wait(o_done + t, (cnt - 1) & 1, dead, AT_O);  // O_t is complete, P_t read
         // (the barrier also keeps P_t, where it lies over S_t, behind both halves' loads)
         if (at_any(id, j == jt || top > m + stale)) {
           *mine = top;
@@ -418,7 +465,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             const float f = raise ? ex2_approx((m - top) * c) : 1.f;
             m = raise ? top : m;
             l = at_total(l) * f;
-            for (int i = half; i < ksteps; i += 2) {
+            for (int i = half; live && i < ksteps; i += 2) {
               float o[16];
               tmem_ld16(to + 16 * i, o);
 #pragma unroll
@@ -430,10 +477,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         // an infinite score makes the row NaN, as inf - inf would
         const float mc = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m * c;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        at_turn_wait(t);
+        if (!Twin || g.turns) at_turn_wait(t);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t p[16];
+          if (!live) break;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 y = __ffma2_rn(make_float2(s[32 * i + 2 * e], s[32 * i + 2 * e + 1]), make_float2(c, c),
@@ -444,31 +492,32 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             p[e] = at_pack<T>(v.x, v.y);
           }
           tmem_st16u(tp + 16 * i, p);
-          if (i == 0) at_turn_give(t);
+          if (i == 0 && (!Twin || g.turns)) at_turn_give(t);
         }
+        if (Twin && !live && g.turns) at_turn_give(t);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_ready + t);
         ++cnt;
       }
-      if (g.twin && t == 1 && n % 2 == 1) {  // tile 0 had one key tile more
+      if (Twin && g.turns && t == 1 && n % 2 == 1) {  // tile 0 had one key tile more
         at_turn_wait(t);
         at_turn_give(t);
       }
       // ---- the unit's rows: to the output when the unit is whole, else to the workspace
       if (any) {
-        at_wait(o_done + t, (cnt - 1) & 1, dead);
+        at_wait(o_done + t, (cnt - 1) & 1, dead, AT_O);
         tc_fence_after();
       }
       *mine = l;
       at_sync(id);
       l = at_total(half ? *other + l : l + *other);
-      if (!g.twin && n == g.tiles) {
+      if (!Twin && n == g.tiles) {
         // through the Q tile, whose products are complete: 16-byte chunks of whole rows,
         // `wide` lanes a row, as Q was read
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        for (int i = half; i < ksteps; i += 2) {
+        for (int i = half; live && i < ksteps; i += 2) {
           float v[16];
           tmem_ld16(to + 16 * i, v);
           uint32_t w[8];
@@ -496,9 +545,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       } else {
         // the piece is kept channel by channel, so that a warp stores 32 rows side by side
         const long piece = 2L * blockIdx.x + (x == x0 ? 0 : 1);
-        if (half == 0) g.part_ml[piece * 256 + 128 * t + row] = make_float2(m == -INFINITY ? m : m * c, l);
-        float* o = g.part + piece * 256 * d + 128 * t + row;
-        for (int i = half; i < ksteps; i += 2) {
+        const int col = Twin ? 128 * t + unit_row : unit_row;
+        if (half == 0) g.part_ml[piece * 256 + col] = make_float2(m == -INFINITY ? m : m * c, l);
+        float* o = g.part + piece * 256 * d + col;
+        for (int i = half; live && i < ksteps; i += 2) {
           float v[16];
           if (any) tmem_ld16(to + 16 * i, v);
 #pragma unroll
@@ -511,7 +561,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       base += (uint32_t)n;
       x += n;
     }
-    if (t == 0) at_turn_wait(t);  // the other tile's last
+    if ((!Twin || g.turns) && t == 0) at_turn_wait(t);  // the other tile's last
   }
   tc_fence_before();
   __syncthreads();
@@ -536,10 +586,10 @@ __global__ void __launch_bounds__(AT_JOIN) attn_join_kernel(const __grid_constan
   const long t0 = unit * g.tiles, c0 = at_owner(g, t0, grid), c1 = at_owner(g, t0 + g.tiles - 1, grid);
   if (c0 == c1 && !g.twin) return;  // written by its CTA
   const int subs = g.twin ? 2 : 1;
-  const int pieces = (int)(c1 - c0 + 1) * subs;
-  const auto piece = [&](int i) {
-    const long cta = c0 + i / subs;
-    return 2 * cta + (at_start(g, cta, grid) >= t0 ? 0 : 1);
+  const int pieces = g.twin ? 2 * g.cuts : (int)(c1 - c0 + 1);
+  const auto piece = [&](int i) -> long {
+    if (g.twin) return 2 * (unit + g.units * (i / 2));
+    return 2 * (c0 + i) + (at_start(g, c0 + i, grid) >= t0 ? 0 : 1);
   };
   float top = -INFINITY;
   for (int i = 0; i < pieces; ++i) top = fmaxf(top, g.part_ml[piece(i) * 256 + 128 * (i % subs) + row].x);

@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <initializer_list>
 #include <string>
+#include <type_traits>
 
 #include "../../include/scunet_b200.h"
 #include "host_logic.h"
@@ -325,7 +326,7 @@ bool attn_tma_ok(const scb_rows& t, int64_t b, int64_t lk, int hk) {
 struct AttnPlan {
   int twin, unit_rows, share;
   long rows, row_units, units, tiles, total;
-  int grid;
+  int grid, cuts;
   bool cut;
   size_t work;
 };
@@ -341,10 +342,16 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
   p.total = p.units * p.tiles;
   long grid = p.units;
   const long waves = (p.units + sms - 1) / sms;
-  if (p.units < sms) {
+  if (p.twin) {
+    // as many pieces as one round of CTAs holds (a second round measured 50 % slower), each
+    // of two tiles or more
+    const long most = p.tiles / 2, s = sms / p.units;
+    p.cuts = (int)(s < 1 ? 1 : s < most ? s : most);
+    grid = p.units * p.cuts;
+  } else if (p.units < sms) {
     const long most = p.total / 4;  // at least four tiles a CTA
     grid = most < p.units ? p.units : most < sms ? most : sms;
-  } else if (!p.twin && p.units < waves * sms * 95 / 100) {
+  } else if (p.units < waves * sms * 95 / 100) {
     grid = sms;
   }
   p.grid = (int)(grid < kMaxBlocks ? grid : kMaxBlocks);
@@ -353,10 +360,10 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
   return p;
 }
 
-template <typename T, int Boxes>
+template <typename T, int Boxes, bool Twin>
 int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk, const CUtensorMap& tv,
                    cudaStream_t st) {
-  const auto kernel = attn_tc_kernel<T, Boxes>;
+  const auto kernel = attn_tc_kernel<T, Boxes, Twin>;
   constexpr int smem = AtLayout<Boxes>::kSmem;
   static std::atomic<uint64_t> raised{0};
   const cudaError_t e = allow_smem((const void*)kernel, smem, raised);
@@ -547,8 +554,9 @@ int scb_rotate_axes(const scb_heads* q, const scb_heads* k, int dtype, int64_t b
     g.items = (unsigned)g.vecs * (unsigned)(g.t[0].heads + g.t[1].heads);
     if (!g.items) return SCB_OK;
     if ((uint64_t)g.vecs * (uint64_t)(g.t[0].heads + g.t[1].heads) > 1u << 24) return refuse(op, "heads too many or too wide");
-    // tokens of a block: four items a thread, but blocks for every SM; angles of at most 32 KB
-    long per = (4L * ROT_THREADS + g.items - 1) / g.items;
+    // tokens of a block: eight items a thread (4 and 16 measured 3 and 5 % slower on wide heads), but
+    // blocks for every SM; angles of at most 32 KB
+    long per = (8L * ROT_THREADS + g.items - 1) / g.items;
     const int sms = sm_count();
     if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
     const long share = (g.tokens + 2L * sms - 1) / (2L * sms);
@@ -640,13 +648,14 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
       const int sms = sm_count();
       if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
       const AttnPlan p = attn_plan(b, lq, lk, h, hk, d, sms);
-      if (p.units <= kMaxBlocks / 256) {
+      if (p.units <= kMaxBlocks / 256 && p.grid > 0) {
         if (p.work && (!work || work_bytes < p.work || addr(work) % 16))
           return refuse(op, "the workspace is too small or not 16-byte aligned (scb_attention_workspace)");
         AttnTcArgs g{};
         g.a = a;
-        g.share = p.share; g.rows = p.rows; g.twin = p.twin; g.unit_rows = p.unit_rows; g.row_units = p.row_units;
+        g.share = p.share; g.rows = p.rows; g.twin = p.twin; g.unit_rows = p.unit_rows; g.cuts = p.cuts; g.row_units = p.row_units;
         g.units = p.units; g.tiles = p.tiles; g.total = p.total;
+        g.turns = p.rows > 64;  // fewer rows leave the special function units idle anyway
         g.kv_b = (b > 1 && k->sb ? 1 : 0) | (b > 1 && v->sb ? 2 : 0);
         g.kv_h = (hk > 1 && k->sh ? 1 : 0) | (hk > 1 && v->sh ? 2 : 0);
         g.qneg = scale < 0 ? 1 : a.scale_log2 == 0 ? 2 : 0;
@@ -661,10 +670,15 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
         CUtensorMap tk, tv;
         if (!attn_map(&tk, *k, dtype, b, lk, hk, d) || !attn_map(&tv, *v, dtype, b, lk, hk, d))
           return global_error(SCB_ECUDA, "scb_attention: no tensor map for k or v");
-        if (dtype == SCB_F16)
-          return d <= 64 ? attn_tc_launch<__half, 1>(g, p, tk, tv, st) : attn_tc_launch<__half, 2>(g, p, tk, tv, st);
-        return d <= 64 ? attn_tc_launch<__nv_bfloat16, 1>(g, p, tk, tv, st)
-                       : attn_tc_launch<__nv_bfloat16, 2>(g, p, tk, tv, st);
+        const auto boxes = [&](auto type, auto twin) {
+          using T = decltype(type);
+          return d <= 64 ? attn_tc_launch<T, 1, decltype(twin)::value>(g, p, tk, tv, st)
+                         : attn_tc_launch<T, 2, decltype(twin)::value>(g, p, tk, tv, st);
+        };
+        const auto typed = [&](auto type) {
+          return p.twin ? boxes(type, std::true_type{}) : boxes(type, std::false_type{});
+        };
+        return dtype == SCB_F16 ? typed(__half{}) : typed(__nv_bfloat16{});
       }
     }
     const long blocks = (lq + ATTN_ANY_WARPS - 1) / ATTN_ANY_WARPS;
