@@ -8,8 +8,9 @@
 //   dx = rstd (h - E_g[h] - xh E_g[h xh]).
 //
 // Two forms, each with its gradient:
-//  * norm_small_kernel: a picture's rows of a few whole groups fit in one block's shared
-//    memory; the values are read once, one launch.
+//  * norm_small_kernel: a picture's rows of a few whole groups fit in the shared memory of a
+//    block, or of a cluster of up to eight that share the rows and read one another's sums
+//    there; the values are read once, one launch.
 //  * norm_stats_kernel, then norm_apply_kernel (norm_grad_sums_kernel, then
 //    norm_grad_apply_kernel): blocks take rows of all pictures and leave one partial per
 //    group; the second launch starts while the first one ends and every block joins its
@@ -34,8 +35,9 @@ struct NormGeom {
   int tc, rp;         // vectors of a row that one block takes (a chunk), rows it takes at once
   int chunks, slots;  // chunks of a row; groups + chunks - 1 partials of a split: a chunk's
                       // part of a group is slot group + chunk (a group may span chunks)
-  int splits;         // row ranges of a picture
+  int splits;         // parts of a picture's rows
   long cycles;        // l / (rp * splits)
+  long range;         // small form: rows of a block
   int whole;          // a vector never spans two groups
   long x_sn, x_sl;    // element strides of pictures and rows
   long y_sn, y_sl;
@@ -56,7 +58,8 @@ struct Moments {
 };
 __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
   const float n = a.n + b.n;
-  if (n == 0.f) return a;
+  if (a.n == 0.f) return b;
+  if (b.n == 0.f) return a;
   const float d = b.mean - a.mean, f = __fdividef(b.n, n);
   return {n, a.mean + d * f, a.m2 + b.m2 + d * d * a.n * f};
 }
@@ -771,8 +774,20 @@ __global__ void __launch_bounds__(1024) norm_grad_params_kernel(const float2* __
   }
 }
 
-// The small form: block (picture, chunk of whole groups), the chunk's values in shared
-// memory; kT threads: 128 where the values are few and blocks many, else 512. GRAD: x and dy, dx out; the channels' sums go to dw and db when there is one
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float2 at `p` of this block's shared memory, in the cluster's block `rank`.
+__device__ __forceinline__ float2 cluster_read(const float2* p, int rank) {
+  uint32_t a;
+  float2 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+// The small form: cluster (picture, chunk of whole groups), of `splits` blocks that take a
+// range of the rows each; the chunk's values in shared memory; kT threads: 128 where the values are few and blocks many, else 512. GRAD: x and dy, dx out; the channels' sums go to dw and db when there is one
 // picture, else to cpart.
 template <typename T, int V, bool GRAD, int kT>
 __global__ void __launch_bounds__(kT)
@@ -781,26 +796,29 @@ norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
                   float* __restrict__ dweight, float* __restrict__ dbias, float2* __restrict__ cpart,
                   const __grid_constant__ NormGeom g) {
   extern __shared__ __align__(16) float norm_sm[];
-  // the block's sums; K; (mean, rstd), (E[h], E[h xh]) of the groups; the values
+  // the block's sums; K; (mean, rstd), (E[h], E[h xh]), shared sums of the groups; the values
   float* first = norm_sm + BlockSums<V, kT>::floats(g.tc);
   float2* stats = reinterpret_cast<float2*>(first + (g.tc * V + 1) / 2 * 2);
   const NormPlace p(g, V);
   const int g0 = p.c0 / g.cpg, ng = (p.c1 - p.c0) / g.cpg;
+  float2* share = stats + 2 * ng;  // what the cluster's blocks read of one another, by group
   Pack<T, V>* keep = reinterpret_cast<Pack<T, V>*>(norm_sm + g.keep);
-  Pack<T, V>* keep_d = keep + (GRAD ? g.l * g.tc : 0);
-  const int t = threadIdx.x % g.tc;
-  const T* src = x + p.pic * g.x_sn + (long)p.col * V;
-  const T* del = GRAD ? dy + p.pic * g.d_sn + (long)p.col * V : nullptr;
-  if (!GRAD) {
+  Pack<T, V>* keep_d = keep + (GRAD ? g.range * g.tc : 0);
+  const int t = threadIdx.x - p.lane * g.tc;
+  const long r0 = min(p.split * g.range, g.l), rows = min(g.range, g.l - r0);  // the block's
+  const T* src = x + p.pic * g.x_sn + r0 * g.x_sl + (long)p.col * V;
+  T* dst = y + p.pic * g.y_sn + r0 * g.y_sl + (long)p.col * V;
+  const float inv = 1.f / ((float)g.l * (float)g.cpg);
+  if constexpr (!GRAD) {
     float k[V], sum[V], sq[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) k[i] = sum[i] = sq[i] = 0.f;
-    if (p.on && g.l > 0) {
+    if (p.on && rows > 0) {
       Pack<T, V> a;
       float v[V];
-      middle_of_rows<T, V>(src, g.x_sl, g.l, k);
+      middle_of_rows<T, V>(src, g.x_sl, rows, k);
 #pragma unroll 4
-      for (long row = p.lane; row < g.l; row += g.rp) {
+      for (long row = p.lane; row < rows; row += g.rp) {
         a.load(src + row * g.x_sl);
         keep[row * g.tc + t] = a;
         unpack(a, v);
@@ -814,41 +832,50 @@ norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
     BlockSums<V, kT> sums;
     sums.add(norm_sm, g, sum, sq, p.lane);
     for (int n = threadIdx.x >> 5; n < ng; n += kT / 32) {
-      const float2 m = group_moments(sums, first, n * g.cpg, (n + 1) * g.cpg, (float)g.l);
-      if ((threadIdx.x & 31) == 0) {
-        const float rs = 1.f / sqrtf((g.l > 0 ? m.y / ((float)g.l * (float)g.cpg) : 0.f) + g.eps);
-        stats[n] = make_float2(m.x, rs);
-        if (mean) mean[p.pic * g.groups + g0 + n] = m.x;
+      const float2 m = group_moments(sums, first, n * g.cpg, (n + 1) * g.cpg, (float)rows);
+      if ((threadIdx.x & 31) == 0) share[n] = m;
+    }
+    g.splits > 1 ? cluster_sync() : __syncthreads();
+    for (int n = threadIdx.x; n < ng; n += kT) {
+      Moments m{0.f, 0.f, 0.f};
+      for (int r = 0; r < g.splits; ++r) {
+        const float2 v = g.splits > 1 ? cluster_read(share + n, r) : share[n];
+        const long from = min(r * g.range, g.l);
+        m = join(m, Moments{(float)min(g.range, g.l - from) * (float)g.cpg, v.x, v.y});
+      }
+      const float rs = 1.f / sqrtf((g.l > 0 ? m.m2 * inv : 0.f) + g.eps);
+      stats[n] = make_float2(m.mean, rs);
+      if (p.split == 0) {
+        if (mean) mean[p.pic * g.groups + g0 + n] = m.mean;
         if (rstd) rstd[p.pic * g.groups + g0 + n] = rs;
       }
     }
-  } else {
-    grad_stats(g, stats, g0, p.c1, mean, rstd, p.pic);
-  }
-  __syncthreads();
-  Channels<V> ch;
-  Hats<V> hat;
-  if (p.on) {
-    ch.load(g, stats, g0, p.col * V, weight, bias);
-    if (GRAD) hat.load(g, stats, g0, p.col * V);
-  }
-  T* dst = y + p.pic * g.y_sn + (long)p.col * V;
-  if constexpr (!GRAD) {
-    if (p.on)
-      for (long row = p.lane; row < g.l; row += g.rp) {
+    __syncthreads();
+    if (p.on) {
+      Channels<V> ch;
+      ch.load(g, stats, g0, p.col * V, weight, bias);
+      for (long row = p.lane; row < rows; row += g.rp) {
         float v[V];
         unpack(keep[row * g.tc + t], v);
         ch.z(v, v);
         act_all<ACT_ANY, V>(g, v);
         repack<T, V>(v).store(dst + row * g.y_sl);
       }
+    }
   } else {
+    const T* del = dy + p.pic * g.d_sn + r0 * g.d_sl + (long)p.col * V;
+    grad_stats(g, stats, g0, p.c1, mean, rstd, p.pic);
+    __syncthreads();
+    Channels<V> ch;
+    Hats<V> hat;
     float sa[V], sb[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.f;
     if (p.on) {
+      ch.load(g, stats, g0, p.col * V, weight, bias);
+      hat.load(g, stats, g0, p.col * V);
 #pragma unroll 2
-      for (long row = p.lane; row < g.l; row += g.rp) {
+      for (long row = p.lane; row < rows; row += g.rp) {
         Pack<T, V> a, e;
         a.load(src + row * g.x_sl);
         e.load(del + row * g.d_sl);
@@ -868,23 +895,30 @@ norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
         const float w = weight ? weight[c] : 1.f;
         m = join(m, make_float2(w * s.x, w * s.y));
         if (cpart) {
-          cpart[p.pic * g.c + c] = s;
+          cpart[(long)blockIdx.x * g.c + c] = s;
         } else {
           if (dbias) dbias[c] = s.x;
           if (dweight) dweight[c] = s.y;
         }
       }
       m = warp_join(m);
-      const float inv = 1.f / ((float)g.l * (float)g.cpg);
-      if ((threadIdx.x & 31) == 0) means[k] = make_float2(m.x * inv, m.y * inv);
+      if ((threadIdx.x & 31) == 0) share[k] = m;
+    }
+    g.splits > 1 ? cluster_sync() : __syncthreads();
+    for (int k = threadIdx.x; k < ng; k += kT) {
+      float2 m = make_float2(0.f, 0.f);
+      for (int r = 0; r < g.splits; ++r) m = join(m, g.splits > 1 ? cluster_read(share + k, r) : share[k]);
+      means[k] = make_float2(m.x * inv, m.y * inv);
     }
     __syncthreads();
-    if (!p.on) return;
-    GradMeans<V> m;
-    m.load(g, hat, means, g0, p.col * V);
-    for (long row = p.lane; row < g.l; row += g.rp)
-      grad_x<T, V, ACT_ANY>(g, ch, hat, m, keep[row * g.tc + t], keep_d[row * g.tc + t]).store(dst + row * g.y_sl);
+    if (p.on) {
+      GradMeans<V> m;
+      m.load(g, hat, means, g0, p.col * V);
+      for (long row = p.lane; row < rows; row += g.rp)
+        grad_x<T, V, ACT_ANY>(g, ch, hat, m, keep[row * g.tc + t], keep_d[row * g.tc + t]).store(dst + row * g.y_sl);
+    }
   }
+  if (g.splits > 1) cluster_sync();  // the others may still be reading this block's sums
 }
 
 }  // namespace scb

@@ -77,26 +77,32 @@ NormPlan norm_plan(NormGeom g, int vec, int es, bool grad, int sms) {
   // some work for a block
   int unit = g.cpg;
   while (unit % vec) unit += g.cpg;
-  // sums and segments, K, four floats a group; then the values
+  // sums and segments, K, six floats a group; then the values
   const auto keep = [&](long cc, int threads) {
     const long segs = cc > threads ? cc : threads;
-    return (2L * vec * threads + 2 * segs + (cc + 1) / 2 * 2 + 4 * (cc / g.cpg) + 3) / 4 * 4;
+    return (2L * vec * threads + 2 * segs + (cc + 1) / 2 * 2 + 6 * (cc / g.cpg) + 3) / 4 * 4;
   };
-  const auto bytes = [&](long cc) { return (double)g.l * cc * es * bufs; };
-  const auto fits = [&](long cc) { return cc <= 512L * vec && 4.0 * keep(cc, 512) + bytes(cc) <= 226 * 1024; };
-  if (fits(unit)) {
+  const auto bytes = [&](long cc, int parts) { return (double)((g.l + parts - 1) / parts) * cc * es * bufs; };
+  const auto fits = [&](long cc, int parts) {
+    return cc <= 512L * vec && 4.0 * keep(cc, 512) + bytes(cc, parts) <= 226 * 1024;
+  };
+  if (fits(unit, 8)) {
     long cc = unit;
-    while (cc < g.c && fits(cc + unit) && (cc * es < 64 || bytes(cc) < 8192)) cc += unit;
+    while (cc < g.c && fits(cc + unit, 8) && (cc * es < 64 || bytes(cc, 1) < 8192)) cc += unit;
+    g.chunks = (int)((g.c + cc - 1) / cc);
+    // blocks of a cluster: as many as the values need; more while a block holds over 16 KB and
+    // SMs are free
+    int parts = 1;
+    while (!fits(cc, parts) || (parts < 8 && bytes(cc, parts) > 16384 && 2 * parts * g.n * g.chunks <= sms)) parts *= 2;
     p.small = true;
-    p.threads = bytes(cc) <= 16384 && cc <= 128L * vec ? 128 : 512;
+    p.threads = bytes(cc, parts) <= 16384 && cc <= 128L * vec ? 128 : 512;
     g.tc = (int)(cc / vec);
     g.rp = p.threads / g.tc;
-    g.chunks = (int)((g.c + cc - 1) / cc);
-    g.splits = 1;
-    g.cycles = g.l / g.rp;
+    g.splits = parts;
+    g.range = (g.l + parts - 1) / parts;
     g.keep = (int)keep(cc, p.threads);
-    p.smem = 4 * (size_t)g.keep + (size_t)g.l * cc * es * bufs;
-    p.cpart = grad && g.n > 1 ? (size_t)g.n * g.c : 0;
+    p.smem = 4 * (size_t)g.keep + (size_t)g.range * cc * es * bufs;
+    p.cpart = grad && g.n * parts > 1 ? (size_t)g.n * parts * g.c : 0;
     p.g = g;
     return p;
   }
@@ -197,9 +203,19 @@ void norm_small(const NormPlan& p, const NormArgs& a) {
   const auto kernel = norm_small_kernel<T, V, GRAD, kT>;
   static std::atomic<uint64_t> raised{0};
   if (allow_smem((const void*)kernel, 227 * 1024, raised) != cudaSuccess) return;  // reported by launched()
-  kernel<<<dim3((unsigned)p.g.n, (unsigned)p.g.chunks), kT, p.smem, a.st>>>(
-      static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<T*>(a.y), a.mean, a.rstd, a.weight, a.bias,
-      a.dweight, a.dbias, p.cpart ? a.cpart : nullptr, p.g);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.g.n * p.g.splits), (unsigned)p.g.chunks);
+  cfg.blockDim = dim3(kT);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = a.st;
+  cudaLaunchAttribute cluster[1];
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim.x = (unsigned)p.g.splits;
+  cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+  cfg.attrs = cluster;
+  cfg.numAttrs = p.g.splits > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<T*>(a.y), a.mean,
+                     a.rstd, a.weight, a.bias, a.dweight, a.dbias, p.cpart ? a.cpart : nullptr, p.g);
 }
 
 // Floats, rounded up to 16 bytes.

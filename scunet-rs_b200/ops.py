@@ -45,7 +45,7 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 def _call(t, fn, *args):
     """fn(*args, stream) on the current stream of t's device; a failure raises its message."""
-    index = t.device.index
+    index = t.get_device()
     if index == torch.cuda.current_device():
         rc = fn(*args, _stream(index))
     else:
@@ -67,10 +67,10 @@ def _work_bytes(name, device, *sizes):
 
 def _workspace(name, t, *sizes):
     """(tensor to keep until the call is launched, its address, its bytes)"""
-    need = _work_bytes(name, t.device.index, *sizes)
+    need = _work_bytes(name, t.get_device(), *sizes)
     if not need:
         return None, None, 0
-    work = torch.empty(need, dtype=torch.uint8, device=t.device)
+    work = t.new_empty(need, dtype=torch.uint8)
     return work, work.data_ptr(), need
 
 
@@ -84,7 +84,7 @@ def _dtype(t, what):
 
 
 def _same(t, like, what):
-    if t.dtype != like.dtype or t.device != like.device or t.shape != like.shape:
+    if t.dtype != like.dtype or t.get_device() != like.get_device() or t.shape != like.shape:
         _fail(f"{what} must be {tuple(like.shape)} {like.dtype} on {like.device}, "
               f"not {tuple(t.shape)} {t.dtype} on {t.device}")
 
@@ -92,7 +92,7 @@ def _same(t, like, what):
 def _params(t, c, like, what):
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.device != like.device or t.shape != (c,) or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.get_device() != like.get_device() or t.shape != (c,) or not t.is_contiguous():
         _fail(f"{what} must be {c} contiguous float32 values on {like.device}")
     return t.data_ptr()
 
@@ -150,7 +150,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act="none", out=N
     yn, yl = (l * c, c) if out is None else _rows(y, "out")[3:]
     mean = rstd = None
     if stats:
-        mean, rstd = (torch.empty((n, max(groups, 1)), dtype=torch.float32, device=x.device) for _ in range(2))
+        mean, rstd = (x.new_empty((n, max(groups, 1)), dtype=torch.float32) for _ in range(2))
     _work, work, size = _workspace("scb_group_norm_workspace", x, n, l, c, groups)
     _call(x, _library().scb_group_norm, x.data_ptr(), sn, sl, dt, n, l, c, groups, _params(weight, c, x, "weight"),
           _params(bias, c, x, "bias"), eps, _act(act), y.data_ptr(), yn, yl, _ptr(mean), _ptr(rstd), work, size)
@@ -168,10 +168,10 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, ac
     dx = _out(out, x)
     xn, xl = (l * c, c) if out is None else _rows(dx, "out")[3:]
     for t, what in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype != torch.float32 or t.device != x.device or t.shape != (n, groups) or not t.is_contiguous():
+        if t.dtype != torch.float32 or t.get_device() != x.get_device() or t.shape != (n, groups) \
+                or not t.is_contiguous():
             _fail(f"{what} must be contiguous float32 [{n}, {groups}] on {x.device}")
-    dparams = torch.empty((2, c), dtype=torch.float32, device=x.device)
-    dw, db = dparams.unbind(0)
+    dw, db = x.new_empty(c, dtype=torch.float32), x.new_empty(c, dtype=torch.float32)
     _work, work, size = _workspace("scb_group_norm_workspace", x, n, l, c, groups)
     _call(x, _library().scb_group_norm_backward, dy.data_ptr(), dn, dl, x.data_ptr(), sn, sl, dt, n, l, c, groups,
           mean.data_ptr(), rstd.data_ptr(), _params(weight, c, x, "weight"), _params(bias, c, x, "bias"), _act(act),
@@ -204,11 +204,11 @@ def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=F
     if q.dim() != 4:
         _fail("q must be [pictures, tokens, heads, channels]")
     b, l, _, d = q.shape
-    if k is not None and (k.dtype != q.dtype or k.device != q.device or k.dim() != 4 or k.shape[:2] != (b, l)
-                          or k.shape[3] != d):
+    if k is not None and (k.dtype != q.dtype or k.get_device() != q.get_device() or k.dim() != 4
+                          or k.shape[:2] != (b, l) or k.shape[3] != d):
         _fail(f"k must be [{b}, {l}, heads, {d}] {q.dtype} on {q.device}")
     axes = len(sections)
-    if positions.dtype not in _POSITIONS or positions.device != q.device:
+    if positions.dtype not in _POSITIONS or positions.get_device() != q.get_device():
         _fail(f"positions must be int32, int64 or float32 on {q.device}")
     if positions.shape == (l, axes):
         pb, (pl, pa) = 0, positions.stride()
@@ -234,7 +234,7 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
     1 / sqrt(d)."""
     dt = _dtype(q, "q")
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4 or t.dtype != q.dtype or t.device != q.device:
+        if t.dim() != 4 or t.dtype != q.dtype or t.get_device() != q.get_device():
             _fail(f"{what} must be [pictures, tokens, heads, channels] {q.dtype} on {q.device}")
         if t.shape[3] > 1 and t.stride(3) != 1:
             _fail(f"{what}: the channels must be contiguous")
@@ -243,7 +243,7 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
     if k.shape != (b, lk, hk, d) or v.shape != k.shape:
         _fail(f"k and v must be [{b}, keys, heads, {d}] alike, not {tuple(k.shape)} and {tuple(v.shape)}")
     if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.device != q.device \
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.get_device() != q.get_device() \
                 or key_mask.shape != (b, lk) or (lk > 1 and key_mask.stride(1) != 1):
             _fail(f"key_mask must be bool or uint8 [{b}, {lk}] on {q.device}, its rows contiguous")
     o = _out(out, q)
