@@ -18,12 +18,13 @@
 //   S_t = Q_t K^T    M 128, N 128, K d        TMEM columns [128 t, +128)
 //   P_t = 2^(c S - c m), 16-bit               64 columns
 //   O_t += P_t V     M 128, N d, K 128        columns [256 + 64 or 128 t, +d), A from TMEM
-// Heads up to 64 wide leave columns for P_t beside S_t, so the next S_t is computed as soon
-// as this one is in registers; with wider heads P_t lies over S_t and the next S_t waits
-// for P_t V. While one tile's softmax runs, the tensor cores compute the other tile's products. The
-// maximum m that a row subtracts is raised only when a tile exceeds it by 2^8 (in P): sums
-// are float32 and P at most 256, so a stale m changes no result, and O, which lives in
-// TMEM, is rescaled only then.
+// Heads up to 64 wide leave columns for P_t beside S_t, and wider ones keep P_t in shared
+// memory, so the next S_t is computed as soon as this one is in registers (Twin with wide
+// heads: P_t lies over S_t, and the next S_t waits for P_t V). While one tile's softmax
+// runs, the tensor cores compute the other tile's products. The maximum m that a row
+// subtracts is raised only when a tile exceeds it by 2^8 (in P): sums are float32 and P at
+// most 256, so a stale m changes no result, and O, which lives in TMEM, is rescaled only
+// then.
 #pragma once
 #include "op_attn.cuh"
 
@@ -129,20 +130,27 @@ __device__ __forceinline__ void at_turn_give(int t) { asm volatile("barrier.cta.
 __device__ __forceinline__ void at_sync(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
 
 // Boxes: 64-channel halves of a head (1 or 2); Slots: K and V tiles in the ring.
-template <int Boxes>
+template <int Boxes, bool Twin>
 struct AtLayout {
   static constexpr int kTile = Boxes * AT_BOX;            // one Q, K or V tile
-  static constexpr int kSlots = Boxes == 1 ? 10 : 5;
+  // Where P_t lies: beside S_t in TMEM for heads up to 64 wide; in shared memory for wider
+  // ones, where S and O fill TMEM, at the price of two ring slots (8160 x 8160 x 8 x 128: 293
+  // us over S_t, 272 us so; where every key is read from DRAM for 256 rows only, 159 and 179
+  // us); over S_t with Twin, whose tiles need the slots
+  static constexpr bool kSharedP = Boxes == 2 && !Twin;
+  static constexpr bool kOwnP = Boxes == 1 || kSharedP;
+  static constexpr int kSlots = Boxes == 1 ? 10 : kSharedP ? 3 : 5;
   static constexpr int kQ = 0;
-  static constexpr int kRing = 2 * kTile;
+  static constexpr int kPTile = 2 * AT_BOX;               // 128 rows x 128 keys
+  static constexpr int kSharedPAt = 2 * kTile;
+  static constexpr int kRing = kSharedPAt + (kSharedP ? 2 * kPTile : 0);
   static constexpr int kBars = kRing + kSlots * kTile;
   // full and empty of every slot, six pairs of barriers, the TMEM address, `dead`
   static constexpr int kRow = kBars + 8 * (2 * kSlots + 12) + 8;  // [2 tiles][2 halves][128] floats
   static constexpr int kSmem = kRow + 2048;
-  // TMEM columns: S_t at 128 t; then O_t, and P_t where there is room for it
-  static constexpr bool kOwnP = Boxes == 1;
+  // TMEM columns: S_t at 128 t; then O_t; P_t (no meaning with kSharedP)
   static constexpr int kO = 256, kOStep = 64 * Boxes;
-  static constexpr int kP = kOwnP ? 384 : 0, kPStep = kOwnP ? 64 : 128;
+  static constexpr int kP = Boxes == 1 ? 384 : 0, kPStep = Boxes == 1 ? 64 : 128;
 };
 
 // One lane of a converged warp. Selecting the issuing thread this way instead of by lane
@@ -186,7 +194,7 @@ template <typename T, int Boxes, bool Twin>
 __global__ void __launch_bounds__(AT_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                const __grid_constant__ AttnTcArgs g) {
-  using L = AtLayout<Boxes>;
+  using L = AtLayout<Boxes, Twin>;
   using Place = AtPlace<Twin, L::kSlots>;
   extern __shared__ __align__(1024) uint8_t sm[];  // the swizzled tiles' alignment
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::kBars);
@@ -262,6 +270,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       constexpr uint32_t id_s = make_idesc_f16(128, 128) | fmt;
       const uint32_t id_o = make_idesc_f16_bmn(128, 16 * ksteps) | fmt;
       const uint64_t dq = make_sdesc(sb + L::kQ + t * L::kTile, 128, SW_128B);
+      const uint64_t dp = make_sdesc(sb + L::kSharedPAt + t * L::kPTile, 128, SW_128B);
       const uint64_t dk = make_sdesc(sb + L::kRing, 128, SW_128B);
       const uint64_t dv = make_sdesc_lbo_sbo(sb + L::kRing, AT_BOX, 1024, SW_128B);
       const uint32_t ts = tmem + 128 * t, tp = tmem + L::kP + L::kPStep * t, to = tmem + L::kO + L::kOStep * t;
@@ -302,7 +311,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           tc_fence_after();
 #pragma unroll
           for (int s = 0; s < AT_KEYS / 16; ++s)
-            umma_f16_ts(to, tp + 8 * s, v + (uint32_t)(2048 * s >> 4), id_o, i > 0 || s > 0);
+            if constexpr (L::kSharedP)
+              umma_f16(to, dp + (uint32_t)(((s >> 2) * AT_BOX + (s & 3) * 32) >> 4), v + (uint32_t)(2048 * s >> 4), id_o,
+                       i > 0 || s > 0);
+            else
+              umma_f16_ts(to, tp + 8 * s, v + (uint32_t)(2048 * s >> 4), id_o, i > 0 || s > 0);
           umma_commit(o_done + t);
           umma_commit(empty + at.slot);
           if (!L::kOwnP && i + 1 < nt) {
@@ -328,6 +341,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const uint32_t ts = trow + 128 * t + 64 * half, to = trow + L::kO + L::kOStep * t;
     const uint32_t tp = trow + L::kP + L::kPStep * t + 32 * half;
     uint8_t* sq = sm + L::kQ + t * L::kTile;
+    uint8_t* sp = sm + L::kSharedPAt + t * L::kPTile + half * AT_BOX;
     float* mine = reinterpret_cast<float*>(sm + L::kRow) + 256 * t + 128 * half + row;
     const float* other = reinterpret_cast<float*>(sm + L::kRow) + 256 * t + 128 * (half ^ 1) + row;
     const float c = g.a.scale_log2, stale = fminf(AT_STALE / c, 1e30f);
@@ -491,12 +505,20 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             sum[e & 1] = __fadd2_rn(sum[e & 1], v);
             p[e] = at_pack<T>(v.x, v.y);
           }
-          tmem_st16u(tp + 16 * i, p);
+          if constexpr (L::kSharedP) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(sp + swz_off(row, 4 * i + k, 128)) =
+                  make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
+          } else {
+            tmem_st16u(tp + 16 * i, p);
+          }
           if (i == 0 && (!Twin || g.turns)) at_turn_give(t);
         }
         if (Twin && !live && g.turns) at_turn_give(t);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_wait_st();
+        if (L::kSharedP) fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(p_ready + t);
         ++cnt;

@@ -380,7 +380,7 @@ template <typename T, int Boxes, bool Twin>
 int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk, const CUtensorMap& tv,
                    cudaStream_t st) {
   const auto kernel = attn_tc_kernel<T, Boxes, Twin>;
-  constexpr int smem = AtLayout<Boxes>::kSmem;
+  constexpr int smem = AtLayout<Boxes, Twin>::kSmem;
   static std::atomic<uint64_t> raised{0};
   const cudaError_t e = allow_smem((const void*)kernel, smem, raised);
   if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
