@@ -208,6 +208,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  let_next_start();
   if (tid == 0) {
     for (int i = 0; i < L::kSlots; ++i) {
       mbar_init(full + i, 1);
@@ -593,53 +594,73 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 
 // Adds the pieces of the units that were cut, 32 rows a block:
 //   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, M the largest m_i
-// A lane is a row (the pieces are stored channel by channel); the result goes through
-// shared memory to be written row by row.
+// A lane is a row (the pieces are stored channel by channel). All maxima and totals are
+// fetched at once and turned into weights in shared memory, then every warp adds its
+// channels, whose loads wait for nothing (piece by piece, each behind its maximum, took 15 to
+// 20 us). The result goes through shared memory to be written row by row.
 constexpr int AT_JOIN = 256;
 template <typename T>
 __global__ void __launch_bounds__(AT_JOIN) attn_join_kernel(const __grid_constant__ AttnTcArgs g, int grid) {
+  extern __shared__ float join_sm[];  // [pieces][32] maxima, later weights; [pieces][32] totals
   __shared__ T out[32][130];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = g.a.d;
+  constexpr int kWarps = AT_JOIN / 32;
   const int groups = g.unit_rows / 32;
   const long unit = blockIdx.x / groups;
-  const int row = (int)(blockIdx.x - unit * groups) * 32 + lane;
-  const long bh = unit / g.row_units, r0 = (unit - bh * g.row_units) * g.unit_rows + row - lane;
+  const int row0 = (int)(blockIdx.x - unit * groups) * 32;
+  const long bh = unit / g.row_units, r0 = (unit - bh * g.row_units) * g.unit_rows + row0;
   if (r0 >= g.rows) return;
   const long t0 = unit * g.tiles, c0 = at_owner(g, t0, grid), c1 = at_owner(g, t0 + g.tiles - 1, grid);
   if (c0 == c1 && !g.twin) return;  // written by its CTA
-  const int subs = g.twin ? 2 : 1;
   const int pieces = g.twin ? 2 * g.cuts : (int)(c1 - c0 + 1);
-  const auto piece = [&](int i) -> long {
-    if (g.twin) return 2 * (unit + g.units * (i / 2));
-    return 2 * (c0 + i) + (at_start(g, c0 + i, grid) >= t0 ? 0 : 1);
+  // piece i: its place among all, in rows; only the first can be its CTA's second
+  const long first = g.twin ? 2 * unit : 2 * c0 + (at_start(g, c0, grid) >= t0 ? 0 : 1);
+  const auto place = [&](int i) -> long {
+    return g.twin ? 2 * (unit + g.units * (i >> 1)) : i == 0 ? first : 2 * (c0 + i);
   };
-  float top = -INFINITY;
-  for (int i = 0; i < pieces; ++i) top = fmaxf(top, g.part_ml[piece(i) * 256 + 128 * (i % subs) + row].x);
-  constexpr int kMost = 128 / (AT_JOIN / 32);  // channels of a warp
-  float o[kMost], l = 0.f;
+  const auto column = [&](int i) { return (g.twin ? 128 * (i & 1) : 0) + row0 + lane; };
+  float *ms = join_sm, *ls = join_sm + 32 * pieces;
+  wait_for_previous();
+  for (int i = warp; i < pieces; i += kWarps) {
+    const float2 ml = __ldcg(g.part_ml + place(i) * 256 + column(i));
+    ms[32 * i + lane] = ml.x;
+    ls[32 * i + lane] = ml.y;
+  }
+  __syncthreads();
+  float top = -INFINITY, l = 0.f;
+  for (int i = 0; i < pieces; ++i) top = fmaxf(top, ms[32 * i + lane]);
+  for (int i = 0; i < pieces; ++i) {
+    const float m = ms[32 * i + lane];
+    l += m == -INFINITY ? 0.f : ex2_approx(m - top) * ls[32 * i + lane];
+  }
+  __syncthreads();
+  for (int i = warp; i < pieces; i += kWarps) {
+    const float m = ms[32 * i + lane];
+    ms[32 * i + lane] = m == -INFINITY ? 0.f : ex2_approx(m - top);
+  }
+  __syncthreads();
+  constexpr int kMost = 128 / kWarps;  // channels of a warp
+  float o[kMost];
 #pragma unroll
   for (int k = 0; k < kMost; ++k) o[k] = 0.f;
+#pragma unroll 2
   for (int i = 0; i < pieces; ++i) {
-    const long p = piece(i);
-    const int col = 128 * (i % subs) + row;
-    const float2 ml = g.part_ml[p * 256 + col];
-    const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-    l += f * ml.y;
-    const float* part = g.part + p * 256 * d + col;
+    const float f = ms[32 * i + lane];
+    const float* part = g.part + place(i) * 256 * d + column(i);
 #pragma unroll
     for (int k = 0; k < kMost; ++k)
-      if (warp + k * (AT_JOIN / 32) < d) {
-        const float v = part[(warp + k * (AT_JOIN / 32)) * 256];
+      if (warp + k * kWarps < d) {
+        const float v = __ldcg(part + (warp + k * kWarps) * 256);
         o[k] += f == 0.f ? 0.f : f * v;
       }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int k = 0; k < kMost; ++k)
-    if (warp + k * (AT_JOIN / 32) < d) out[lane][warp + k * (AT_JOIN / 32)] = from_f32<T>(o[k] * inv);
+    if (warp + k * kWarps < d) out[lane][warp + k * kWarps] = from_f32<T>(o[k] * inv);
   __syncthreads();
   const int b = (int)(bh / g.a.hk), hk = (int)(bh - (long)b * g.a.hk);
-  for (int rr = warp; rr < 32 && r0 + rr < g.rows; rr += AT_JOIN / 32) {
+  for (int rr = warp; rr < 32 && r0 + rr < g.rows; rr += kWarps) {
     const long ql = (r0 + rr) / g.share;
     const long qh = hk * g.share + (r0 + rr - ql * g.share);
     T* dst = static_cast<T*>(g.a.o) + b * g.a.o_sb + ql * g.a.o_sl + qh * g.a.o_sh;

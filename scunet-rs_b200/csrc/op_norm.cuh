@@ -436,11 +436,6 @@ struct NormPlace {
   }
 };
 
-// Launch order of the two passes (programmatic dependent launch): the first lets the second
-// start early, the second waits for the first's results before it reads or writes anything.
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // First pass: per (picture, split, chunk's part of a group) mean and M2.
 template <typename T, int V>
 __global__ void __launch_bounds__(NORM_THREADS, 2)

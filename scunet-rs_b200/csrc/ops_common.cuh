@@ -49,6 +49,12 @@ struct alignas(V * sizeof(T)) Pack {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Pack*>(p) = *this; }
 };
 
+// Launch order of two kernels (programmatic dependent launch): the first lets the second
+// start early, the second waits for the first's results before it reads or writes anything
+// of theirs.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Activations; 0 to 2 number them as the GEMM epilogues do.
 enum : int { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3, ACT_ANY = -1 };
 

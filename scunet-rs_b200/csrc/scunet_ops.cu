@@ -52,6 +52,23 @@ int sm_count() {
   return sms;
 }
 
+// Launch `kernel` so that it may start while the launch before it in the stream ends
+// (it waits for that launch's results itself).
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = a;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // ---------------------------------------------------------------------------- group norm
 const long kMaxBlocks = 0x7fffffffl;
 
@@ -158,23 +175,6 @@ int norm_vec(int es, int c, int most, std::initializer_list<uint64_t> bytes) {
   if (v < 1) return 0;
   while (v > 1 && c % v) v /= 2;
   return v == most / es ? v : v >= 2 ? 2 : 1;
-}
-
-// Launch `kernel` so that it may start while the launch before it in the stream ends
-// (it waits for that launch's results itself).
-template <typename... P, typename... A>
-void launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  a[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = a;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
 // Raises a kernel's shared memory limit, once on each device (`raised`: one per kernel).
@@ -342,7 +342,7 @@ bool attn_tma_ok(const scb_rows& t, int64_t b, int64_t lk, int hk) {
 struct AttnPlan {
   int twin, unit_rows, share;
   long rows, row_units, units, tiles, total;
-  int grid, cuts;
+  int grid, cuts, pieces;  // pieces: of a unit, at most
   bool cut;
   size_t work;
 };
@@ -372,6 +372,7 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
   }
   p.grid = (int)(grid < kMaxBlocks ? grid : kMaxBlocks);
   p.cut = p.grid != p.units;
+  p.pieces = p.twin ? 2 * p.cuts : (int)(p.grid / p.units + 2);
   p.work = p.cut || p.twin ? (size_t)p.grid * 2 * 256 * (d + 2) * sizeof(float) : 0;
   return p;
 }
@@ -385,7 +386,13 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
   const cudaError_t e = allow_smem((const void*)kernel, smem, raised);
   if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
   kernel<<<p.grid, AT_THREADS, smem, st>>>(tk, tv, g);
-  if (p.cut || p.twin) attn_join_kernel<T><<<(unsigned)(p.units * (p.unit_rows / 32)), AT_JOIN, 0, st>>>(g, p.grid);
+  if (p.cut || p.twin) {
+    static std::atomic<uint64_t> raised_join{0};
+    const cudaError_t ej = allow_smem((const void*)attn_join_kernel<T>, 128 * 1024, raised_join);
+    if (ej != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(ej));
+    launch_after(attn_join_kernel<T>, dim3((unsigned)(p.units * (p.unit_rows / 32))), AT_JOIN, (size_t)256 * p.pieces, st,
+                 g, p.grid);
+  }
   return launched("scb_attention");
 }
 
