@@ -452,15 +452,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 #pragma unroll
             for (int i = 0; i < 64; ++i) s[i] = seen[i >> 5] >> (i & 31) & 1 ? s[i] : -INFINITY;
           }
-          if (mask) {
+          if (mask && (Twin || t == 0)) {
             // hidden values may be NaN or infinite, and 0 times those is NaN: clear this
-            // half's hidden rows of V, 64 threads each half of a row's chunks or boxes
+            // half's hidden rows of V. (Tile 1 reads the same V, without Twin, and comes after
+            // tile 0 in their turns.) Two threads a row, each with a box or every other chunk;
+            // neighbouring rows start at different chunks, that is, banks
             const Place at(2 * (base + (uint32_t)(j - (int)j0)) + 1);
             at_wait(full + at.slot, at.turn & 1, dead, AT_FULL);
             if (!((row & 32 ? seen[1] : seen[0]) >> (row & 31) & 1)) {
-              uint4* v = reinterpret_cast<uint4*>(sm + L::kRing + at.slot * L::kTile + (64 * half + (row & 63)) * 128 +
-                                                  (row >> 6) * (Boxes == 2 ? AT_BOX : 64));
-              for (int k = 0; k < 4 * Boxes; ++k) v[k] = make_uint4(0, 0, 0, 0);
+              uint4* v = reinterpret_cast<uint4*>(sm + L::kRing + at.slot * L::kTile + (64 * half + (row & 63)) * 128);
+              const int part = row >> 6;
+              for (int k = 0; k < 4 * Boxes; ++k)
+                v[Boxes == 2 ? part * (AT_BOX / 16) + ((k + row) & 7) : (2 * k + part + row) & 7] = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
           }
