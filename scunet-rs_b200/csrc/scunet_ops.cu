@@ -168,13 +168,13 @@ int norm_check(const char* op, int dtype, int64_t n, int64_t l, int c, int group
   return SCB_OK;
 }
 
-// The widest access that every row of every tensor allows: `most` bytes, two elements, one.
+// Elements of the widest access, `most` bytes at most, that every row of every tensor allows.
 int norm_vec(int es, int c, int most, std::initializer_list<uint64_t> bytes) {
   const int a = common_alignment(most, bytes);
   int v = a / es;
   if (v < 1) return 0;
   while (v > 1 && c % v) v /= 2;
-  return v == most / es ? v : v >= 2 ? 2 : 1;
+  return v;
 }
 
 // Raises a kernel's shared memory limit, once on each device (`raised`: one per kernel).
@@ -396,18 +396,20 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
   return launched("scb_attention");
 }
 
-// F<T, V>() for the element type and vector width: 16 bytes, 4 (the gradient's 16-bit types
-// where groups are not multiples of 8 wide), 2 or 1 elements.
-#define NORM_16(T, vec, F, mid, ...) \
-  (vec == 8 ? F<T, 8>(__VA_ARGS__) : mid && vec == 4 ? F<T, 4>(__VA_ARGS__) : vec == 2 ? F<T, 2>(__VA_ARGS__) : F<T, 1>(__VA_ARGS__))
-#define NORM_DISPATCH(dtype, vec, F, mid, ...)                                                                          \
-  do {                                                                                                                \
-    if (dtype == SCB_F32)                                                                                             \
-      vec == 4 ? F<float, 4>(__VA_ARGS__) : vec == 2 ? F<float, 2>(__VA_ARGS__) : F<float, 1>(__VA_ARGS__);           \
-    else if (dtype == SCB_F16)                                                                                        \
-      NORM_16(__half, vec, F, mid, __VA_ARGS__);                                                                      \
-    else                                                                                                              \
-      NORM_16(__nv_bfloat16, vec, F, mid, __VA_ARGS__);                                                               \
+// F<T, V>() for the element type and vector width.
+#define NORM_16(T, vec, F, ...)                                                                              \
+  (vec == 8   ? F<T, 8>(__VA_ARGS__)                                                                         \
+   : vec == 4 ? F<T, 4>(__VA_ARGS__)                                                                         \
+   : vec == 2 ? F<T, 2>(__VA_ARGS__)                                                                         \
+              : F<T, 1>(__VA_ARGS__))
+#define NORM_DISPATCH(dtype, vec, F, ...)                                                                    \
+  do {                                                                                                       \
+    if (dtype == SCB_F32)                                                                                    \
+      vec == 4 ? F<float, 4>(__VA_ARGS__) : vec == 2 ? F<float, 2>(__VA_ARGS__) : F<float, 1>(__VA_ARGS__);  \
+    else if (dtype == SCB_F16)                                                                               \
+      NORM_16(__half, vec, F, __VA_ARGS__);                                                                  \
+    else                                                                                                     \
+      NORM_16(__nv_bfloat16, vec, F, __VA_ARGS__);                                                           \
   } while (0)
 
 }  // namespace
@@ -458,7 +460,7 @@ int scb_group_norm(const void* x, int64_t x_sn, int64_t x_sl, int dtype, int64_t
     a.x = x; a.y = y; a.mean = mean; a.rstd = rstd; a.weight = weight; a.bias = bias;
     a.part = static_cast<float2*>(work);
     a.st = static_cast<cudaStream_t>(stream);
-    NORM_DISPATCH(dtype, vec, norm_forward, false, p, a);
+    NORM_DISPATCH(dtype, vec, norm_forward, p, a);
     return launched(op);
   });
 }
@@ -502,7 +504,7 @@ int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const vo
     a.part = static_cast<float2*>(work);
     a.cpart = a.part + p.part;
     a.st = st;
-    NORM_DISPATCH(dtype, vec, norm_backward, true, p, a);
+    NORM_DISPATCH(dtype, vec, norm_backward, p, a);
     return launched(op);
   });
 }

@@ -231,7 +231,7 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
     q is [b, lq, h, d], k and v [b, lk, hk, d] with d at most 256; query head i reads key head
     i / (h / hk). key_mask is bool or uint8 [b, lk], nonzero = visible: what hidden keys hold
     does not matter, and queries with no visible key give zeros. scale defaults to
-    1 / sqrt(d)."""
+    1 / sqrt(d). Fast (tensor cores) for d up to 128 and 16-byte aligned rows of k and v."""
     dt = _dtype(q, "q")
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         if t.dim() != 4 or t.dtype != q.dtype or t.get_device() != q.get_device():
