@@ -41,7 +41,8 @@
 namespace scb {
 
 constexpr int AT_KEYS = 128;               // keys of a tile
-constexpr int AT_THREADS = 640;            // launched with 96 registers a thread
+constexpr int AT_THREADS = 640;
+constexpr int AT_REGS = 96;                // registers a thread at launch (checked there)
 constexpr float AT_STALE = 8.f;            // log2 by which a tile may exceed m
 constexpr int AT_BOX = AT_KEYS * 128;      // bytes of 128 rows x 64 channels
 

@@ -351,7 +351,9 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
   p.share = h / hk;
   p.rows = lq * p.share;
   p.tiles = (lk + AT_KEYS - 1) / AT_KEYS;
-  p.twin = p.rows <= 128 && p.tiles > 1;
+  // (twin units always leave pieces, so not for more units than a few rounds of CTAs: the
+  // workspace stays below 160 MB)
+  p.twin = p.rows <= 128 && p.tiles > 1 && b * hk <= 4L * sms;
   p.unit_rows = p.twin ? 128 : 256;
   p.row_units = (p.rows + p.unit_rows - 1) / p.unit_rows;
   p.units = b * hk * p.row_units;
@@ -383,6 +385,15 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
   const auto kernel = attn_tc_kernel<T, Boxes, Twin>;
   constexpr int smem = AtLayout<Boxes, Twin>::kSmem;
   static std::atomic<uint64_t> raised{0};
+  if (!raised.load()) {
+    // the kernel's register split draws on what it is launched with: less would wait forever
+    cudaFuncAttributes fa;
+    const cudaError_t e = cudaFuncGetAttributes(&fa, (const void*)kernel);
+    if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
+    if (fa.numRegs != AT_REGS)
+      return global_error(SCB_ECUDA, "scb_attention: built with " + std::to_string(fa.numRegs) + " registers a thread, not " +
+                                         std::to_string(AT_REGS));
+  }
   const cudaError_t e = allow_smem((const void*)kernel, smem, raised);
   if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
   kernel<<<p.grid, AT_THREADS, smem, st>>>(tk, tv, g);

@@ -476,6 +476,38 @@ def test_attention(torch, ops, b, lq, lk, h, hk, d, dtype):
     check_attention(torch, ops, *qkv_of(torch, b, lq, lk, h, hk, d, dtype_of(torch, dtype)))
 
 
+@pytest.mark.parametrize("b,lq,lk,h,hk,d", [(700, 1, 300, 2, 2, 32), (300, 2, 140, 6, 2, 64), (150, 1, 257, 1, 1, 128),
+                                            (40, 130, 200, 4, 4, 64), (1200, 1, 100, 1, 1, 16)])
+def test_attention_many_pictures(torch, ops, b, lq, lk, h, hk, d):
+    """More pictures and heads than CTAs run at once: several rounds, cut and whole units."""
+    check_attention(torch, ops, *qkv_of(torch, b, lq, lk, h, hk, d, torch.float16, seed=7))
+
+
+def test_attention_free_running_tiles(torch, ops):
+    """One query over many keys, several times: the two key streams of a CTA run freely."""
+    for heads_first in (False, True):
+        q, k, v = qkv_of(torch, 2, 1, 16000, 8, 8, 64, torch.float16, seed=8)
+        if heads_first:
+            k, v = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (k, v))
+        first = ops.attention(q, k, v)
+        check_attention(torch, ops, q, k, v, got=first)
+        assert all(torch.equal(first, ops.attention(q, k, v)) for _ in range(50))
+    ops.status()
+
+
+def test_attention_nan_and_infinity_in_visible_keys(torch, ops):
+    """A NaN key makes every row that sees it NaN, an infinite score too; no other picture."""
+    for lq in (3, 300):
+        for bad in (math.nan, math.inf):
+            for at in (0, 77, 150):
+                q, k, v = qkv_of(torch, 2, lq, 200, 2, 2, 64, torch.float16, seed=9)
+                q = q.abs() + 0.1
+                k[1, at, 0] = bad
+                out = ops.attention(q, k, v)
+                assert torch.isnan(out[1, :, 0]).all() and torch.isfinite(out[0]).all()
+                assert torch.isfinite(out[1, :, 1]).all()
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("b,lq,lk,h,hk,d", [(4, 70, 300, 4, 2, 64), (4, 1, 3000, 2, 2, 128), (4, 200, 130, 2, 1, 32),
                                             (4, 5, 6, 1, 1, 7), (4, 140, 520, 2, 2, 40)])
