@@ -84,7 +84,9 @@ __device__ __forceinline__ void at_range(const AttnTcArgs& g, long cta, long gri
   }
 }
 // The CTA whose range holds tile x.
-__device__ __forceinline__ long at_owner(const AttnTcArgs& g, long x, long grid) { return ((x + 1) * grid - 1) / g.total; }
+__device__ __forceinline__ long at_owner(const AttnTcArgs& g, long x, long grid) {
+  return ((x + 1) * grid - 1) / g.total;
+}
 
 template <typename T>
 __device__ __forceinline__ uint32_t at_pack(float a, float b);
@@ -137,8 +139,12 @@ __device__ __forceinline__ bool at_any(int id, bool p) {
 }
 // The two tiles' exponentials take turns: a tile waits for its turn, and gives the other
 // tile's half-way through its own (512 threads: 256 wait, 256 give).
-__device__ __forceinline__ void at_turn_wait(int t) { asm volatile("barrier.cta.sync %0, 512;" ::"r"(3 + t) : "memory"); }
-__device__ __forceinline__ void at_turn_give(int t) { asm volatile("barrier.cta.arrive %0, 512;" ::"r"(4 - t) : "memory"); }
+__device__ __forceinline__ void at_turn_wait(int t) {
+  asm volatile("barrier.cta.sync %0, 512;" ::"r"(3 + t) : "memory");
+}
+__device__ __forceinline__ void at_turn_give(int t) {
+  asm volatile("barrier.cta.arrive %0, 512;" ::"r"(4 - t) : "memory");
+}
 __device__ __forceinline__ void at_sync(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
 
 // Boxes: 64-channel halves of a head (1 or 2); Slots: K and V tiles in the ring.
@@ -195,7 +201,15 @@ struct AtPlace {
 
 // A bounded wait that gives up at once when another wait of the CTA has given up. The error
 // word tells the place of the first one that did.
-enum : unsigned { AT_EMPTY = 0x100, AT_FULL = 0x200, AT_Q = 0x300, AT_S = 0x400, AT_FREE = 0x500, AT_P = 0x600, AT_O = 0x700 };
+enum : unsigned {
+  AT_EMPTY = 0x100,
+  AT_FULL = 0x200,
+  AT_Q = 0x300,
+  AT_S = 0x400,
+  AT_FREE = 0x500,
+  AT_P = 0x600,
+  AT_O = 0x700,
+};
 __device__ __forceinline__ void at_wait(uint64_t* bar, uint32_t parity, volatile int* dead, unsigned place) {
   if (mbar_try_wait(bar, parity)) return;
   if (*dead) return;
@@ -325,8 +339,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 #pragma unroll
           for (int s = 0; s < AT_KEYS / 16; ++s)
             if constexpr (L::kSharedP)
-              umma_f16(to, dp + (uint32_t)(((s >> 2) * AT_BOX + (s & 3) * 32) >> 4), v + (uint32_t)(2048 * s >> 4), id_o,
-                       i > 0 || s > 0);
+              umma_f16(to, dp + (uint32_t)(((s >> 2) * AT_BOX + (s & 3) * 32) >> 4), v + (uint32_t)(2048 * s >> 4),
+                       id_o, i > 0 || s > 0);
             else
               umma_f16_ts(to, tp + 8 * s, v + (uint32_t)(2048 * s >> 4), id_o, i > 0 || s > 0);
           umma_commit(o_done + t);
@@ -358,7 +372,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     float* mine = reinterpret_cast<float*>(sm + L::kRow) + 256 * t + 128 * half + row;
     const float* other = reinterpret_cast<float*>(sm + L::kRow) + 256 * t + 128 * (half ^ 1) + row;
     const float c = g.a.scale_log2, stale = fminf(AT_STALE / c, 1e30f);
-    const int last = (int)(g.tiles - 1), tail = (int)(g.a.lk - (long)last * AT_KEYS) - 64 * half;  // of the last tile, past this half's first key
+    // the last tile, and its keys from this half's first on
+    const int last = (int)(g.tiles - 1), tail = (int)(g.a.lk - (long)last * AT_KEYS) - 64 * half;
     uint32_t cnt = 0, base = 0;
     if ((!Twin || g.turns) && t == 1) at_turn_give(t);
     for (long x = x0; x < x1;) {
@@ -475,7 +490,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
               uint4* v = reinterpret_cast<uint4*>(sm + L::kRing + at.slot * L::kTile + (64 * half + (row & 63)) * 128);
               const int part = row >> 6;
               for (int k = 0; k < 4 * Boxes; ++k)
-                v[Boxes == 2 ? part * (AT_BOX / 16) + ((k + row) & 7) : (2 * k + part + row) & 7] = make_uint4(0, 0, 0, 0);
+                v[Boxes == 2 ? part * (AT_BOX / 16) + ((k + row) & 7) : (2 * k + part + row) & 7] =
+                    make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
           }

@@ -789,8 +789,9 @@ __device__ __forceinline__ float2 cluster_read(const float2* p, int rank) {
 }
 
 // The small form: cluster (picture, chunk of whole groups), of `splits` blocks that take a
-// range of the rows each; the chunk's values in shared memory; kT threads: 128 where the values are few and blocks many, else 512. GRAD: x and dy, dx out; the channels' sums go to dw and db when there is one
-// picture, else to cpart.
+// range of the rows each; the chunk's values in shared memory; kT threads: 128 where the
+// values are few, else 512. GRAD: x and dy, dx out; the channels' sums go to dw and db when
+// there is one block of them, else to cpart.
 template <typename T, int V, bool GRAD, int kT>
 __global__ void __launch_bounds__(kT)
 norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,

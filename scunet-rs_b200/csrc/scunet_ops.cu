@@ -47,8 +47,8 @@ uint64_t addr(const void* p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); 
 
 int sm_count() {
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
   return sms;
 }
 
@@ -214,8 +214,8 @@ void norm_small(const NormPlan& p, const NormArgs& a) {
   cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
   cfg.attrs = cluster;
   cfg.numAttrs = p.g.splits > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<T*>(a.y), a.mean,
-                     a.rstd, a.weight, a.bias, a.dweight, a.dbias, p.cpart ? a.cpart : nullptr, p.g);
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<T*>(a.y),
+                     a.mean, a.rstd, a.weight, a.bias, a.dweight, a.dbias, p.cpart ? a.cpart : nullptr, p.g);
 }
 
 // Floats, rounded up to 16 bytes.
@@ -391,8 +391,8 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
     const cudaError_t e = cudaFuncGetAttributes(&fa, (const void*)kernel);
     if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
     if (fa.numRegs != AT_REGS)
-      return global_error(SCB_ECUDA, "scb_attention: built with " + std::to_string(fa.numRegs) + " registers a thread, not " +
-                                         std::to_string(AT_REGS));
+      return global_error(SCB_ECUDA, "scb_attention: built with " + std::to_string(fa.numRegs) +
+                                         " registers a thread, not " + std::to_string(AT_REGS));
   }
   const cudaError_t e = allow_smem((const void*)kernel, smem, raised);
   if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
@@ -401,8 +401,8 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
     static std::atomic<uint64_t> raised_join{0};
     const cudaError_t ej = allow_smem((const void*)attn_join_kernel<T>, 128 * 1024, raised_join);
     if (ej != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(ej));
-    launch_after(attn_join_kernel<T>, dim3((unsigned)(p.units * (p.unit_rows / 32))), AT_JOIN, (size_t)256 * p.pieces, st,
-                 g, p.grid);
+    const dim3 blocks((unsigned)(p.units * (p.unit_rows / 32)));
+    launch_after(attn_join_kernel<T>, blocks, AT_JOIN, (size_t)256 * p.pieces, st, g, p.grid);
   }
   return launched("scb_attention");
 }
@@ -497,9 +497,10 @@ int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const vo
     const int es = elem_size(dtype), sms = sm_count();
     if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
     // vectors of 8 only within one group (op_norm.cuh, Hats)
-    const int vec = norm_vec(es, c, es == 2 && c / groups % 8 ? 8 : 16, {addr(x), addr(dy), addr(dx), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
-                                     (uint64_t)(d_sn * es), (uint64_t)(d_sl * es), (uint64_t)(dx_sn * es),
-                                     (uint64_t)(dx_sl * es)});
+    const int vec = norm_vec(es, c, es == 2 && c / groups % 8 ? 8 : 16,
+                             {addr(x), addr(dy), addr(dx), (uint64_t)(x_sn * es), (uint64_t)(x_sl * es),
+                              (uint64_t)(d_sn * es), (uint64_t)(d_sl * es), (uint64_t)(dx_sn * es),
+                              (uint64_t)(dx_sl * es)});
     if (!vec) return refuse(op, "data not aligned to its element size");
     NormGeom g{};
     g.n = n; g.l = l; g.c = c; g.groups = groups; g.act = act;
@@ -589,7 +590,8 @@ int scb_rotate_axes(const scb_heads* q, const scb_heads* k, int dtype, int64_t b
     g.vecs = layout == ROT_INTERLEAVED && vec > 1 ? d / 2 / vec : (d - g.pairs) / vec;
     g.items = (unsigned)g.vecs * (unsigned)(g.t[0].heads + g.t[1].heads);
     if (!g.items) return SCB_OK;
-    if ((uint64_t)g.vecs * (uint64_t)(g.t[0].heads + g.t[1].heads) > 1u << 24) return refuse(op, "heads too many or too wide");
+    if ((uint64_t)g.vecs * (uint64_t)(g.t[0].heads + g.t[1].heads) > 1u << 24)
+      return refuse(op, "heads too many or too wide");
     // tokens of a block: eight items a thread (4 and 16 measured 3 and 5 % slower on wide heads), but
     // blocks for every SM; angles of at most 32 KB
     long per = (8L * ROT_THREADS + g.items - 1) / g.items;
@@ -689,7 +691,8 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
           return refuse(op, "the workspace is too small or not 16-byte aligned (scb_attention_workspace)");
         AttnTcArgs g{};
         g.a = a;
-        g.share = p.share; g.rows = p.rows; g.twin = p.twin; g.unit_rows = p.unit_rows; g.cuts = p.cuts; g.row_units = p.row_units;
+        g.share = p.share; g.rows = p.rows; g.twin = p.twin; g.unit_rows = p.unit_rows; g.cuts = p.cuts;
+        g.row_units = p.row_units;
         g.units = p.units; g.tiles = p.tiles; g.total = p.total;
         g.turns = p.rows > 64;  // fewer rows leave the special function units idle anyway
         g.kv_b = (b > 1 && k->sb ? 1 : 0) | (b > 1 && v->sb ? 2 : 0);

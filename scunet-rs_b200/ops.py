@@ -179,6 +179,12 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, ac
     return dx, dw, db
 
 
+@functools.lru_cache(maxsize=256)
+def _sections(sections):
+    """(C array, pairs) of the axes' sections."""
+    return (ctypes.c_int * len(sections))(*sections), sum(sections)
+
+
 def _heads(x, out, what):
     if x.dim() != 4:
         _fail(f"{what} must be [pictures, tokens, heads, channels]")
@@ -208,6 +214,7 @@ def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=F
                           or k.shape[:2] != (b, l) or k.shape[3] != d):
         _fail(f"k must be [{b}, {l}, heads, {d}] {q.dtype} on {q.device}")
     axes = len(sections)
+    c_sections, pairs = _sections(tuple(sections))
     if positions.dtype not in _POSITIONS or positions.get_device() != q.get_device():
         _fail(f"positions must be int32, int64 or float32 on {q.device}")
     if positions.shape == (l, axes):
@@ -216,12 +223,12 @@ def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=F
         pb, pl, pa = positions.stride()
     else:
         _fail(f"positions must be [{l}, {axes}] or [{b}, {l}, {axes}], not {tuple(positions.shape)}")
-    _params(inv_freq, sum(sections), q, "inv_freq")
+    _params(inv_freq, pairs, q, "inv_freq")
     yq = _out(None if out is None else out[0], q, "out[0]")
     yk = None if k is None else _out(None if out is None else out[1], k, "out[1]")
     _call(q, _library().scb_rotate_axes, _heads(q, yq, "q"), None if k is None else _heads(k, yk, "k"), dt, b, l, d,
           positions.data_ptr(), _POSITIONS[positions.dtype], pb, pl, pa, inv_freq.data_ptr(),
-          (ctypes.c_int * axes)(*sections), axes, SCB_ROT_LAYOUTS[layout], bool(inverse))
+          c_sections, axes, SCB_ROT_LAYOUTS[layout], bool(inverse))
     return yq, yk
 
 
