@@ -625,6 +625,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 
 // Adds the pieces of the units that were cut, 32 rows a block:
 //   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, M the largest m_i
+// A piece without a score for a row (m_i = -inf) weighs nothing, but a NaN in its total, that
+// of a NaN score (maxima skip those), makes the row NaN as it does in an uncut unit.
 // A lane is a row (the pieces are stored channel by channel). All maxima and totals are
 // fetched at once and turned into weights in shared memory, then every warp adds its
 // channels, whose loads wait for nothing (piece by piece, each behind its maximum, took 15 to
@@ -661,8 +663,8 @@ __global__ void __launch_bounds__(AT_JOIN) attn_join_kernel(const __grid_constan
   float top = -INFINITY, l = 0.f;
   for (int i = 0; i < pieces; ++i) top = fmaxf(top, ms[32 * i + lane]);
   for (int i = 0; i < pieces; ++i) {
-    const float m = ms[32 * i + lane];
-    l += m == -INFINITY ? 0.f : ex2_approx(m - top) * ls[32 * i + lane];
+    const float m = ms[32 * i + lane], li = ls[32 * i + lane];
+    l += m != -INFINITY ? ex2_approx(m - top) * li : li == li ? 0.f : li;
   }
   __syncthreads();
   for (int i = warp; i < pieces; i += kWarps) {
