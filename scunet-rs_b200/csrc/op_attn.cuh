@@ -6,6 +6,8 @@
 // One pass over the keys with the running maximum m and sum l of the softmax (in units of
 // log2): when a tile raises m to m', the accumulated o and l are scaled by 2^(m - m').
 #pragma once
+#include <cfloat>
+
 #include "ops_common.cuh"
 
 namespace scb {
@@ -57,7 +59,9 @@ __global__ void __launch_bounds__(32 * ATTN_ANY_WARPS) attn_any_kernel(const Att
     }
     float top = s;
     for (int x = 16; x >= 1; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float m2 = fmaxf(m, top);
+    // (a step whose visible scores are all -inf gets the lowest finite maximum, so that they weigh
+    // nothing beside a finite score of another step; alone they leave l at 0, and 0 / 0 is NaN)
+    const float m2 = fmaxf(fmaxf(m, top), -FLT_MAX);
     const float keep = m == -INFINITY ? 0.f : exp2f(m - m2);
     const float p = seen ? exp2f(s - m2) : 0.f;
     float sum = p;
@@ -76,7 +80,7 @@ __global__ void __launch_bounds__(32 * ATTN_ANY_WARPS) attn_any_kernel(const Att
     }
   }
   T* out = static_cast<T*>(a.o) + b * a.o_sb + i * a.o_sl + h * a.o_sh;
-  const bool none = m == -INFINITY && l == 0.f;
+  const bool none = m == -INFINITY;  // no visible key
 #pragma unroll
   for (int c = 0; c < ATTN_ANY_D / 32; ++c)
     if (lane + 32 * c < a.d) out[lane + 32 * c] = from_f32<T>(none ? 0.f : o[c] / l);

@@ -1,10 +1,37 @@
 """Scores of minus infinity on visible keys, and values that a weight of zero has to remove."""
+import math
+
 import pytest
 
 from test_attention_special_gpu import CUTS, cuts
-from test_ops_gpu import ops, torch  # noqa: F401 (fixtures)
+from test_ops_gpu import check_attention, ops, qkv_of, torch  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
+
+
+def infinite_keys(torch, cut, dt, seed):  # noqa: F811
+    """Queries that are positive in channel 0, so that a key with -inf there scores -inf."""
+    b, lq, lk, h, hk, d = CUTS[cut]
+    q, k, v = qkv_of(torch, b, lq, lk, h, hk, d, dt, seed=seed)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    return q, k, v
+
+
+@cuts
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("finite", ["first", "last", "some"])
+def test_some_scores_minus_infinity(torch, ops, cut, dtype, finite):  # noqa: F811
+    """Such keys weigh nothing where a row has a finite score, as hidden keys do."""
+    q, k, v = infinite_keys(torch, cut, getattr(torch, dtype), 62)
+    lk = k.shape[1]
+    keep = torch.zeros(k.shape[:2], dtype=torch.bool, device="cuda")
+    if finite == "some":
+        keep[:] = torch.arange(lk, device="cuda") % 7 == 5
+    else:
+        keep[:, 0 if finite == "first" else lk - 1] = True
+    bad = torch.where(keep[:, :, None, None], k, torch.tensor(-math.inf, device="cuda", dtype=k.dtype))
+    bad[..., 1:] = k[..., 1:]
+    check_attention(torch, ops, q, k, v, keep, got=ops.attention(q, bad, v))
 
 
 @cuts
