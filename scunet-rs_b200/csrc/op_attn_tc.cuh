@@ -24,7 +24,9 @@
 // runs, the tensor cores compute the other tile's products. The maximum m that a row
 // subtracts is raised only when a tile exceeds it by 2^8 (in P): sums are float32 and P at
 // most 256, so a stale m changes no result, and O, which lives in TMEM, is rescaled only
-// then.
+// then. m is -inf while no key was visible and at least AT_LOWEST after that, so the end can
+// tell rows that see nothing (zeros) from rows whose visible scores are all -inf (0 / 0, NaN):
+// the weights of any other row sum up to 1 or more.
 //
 // Precision: scores, maxima, sums and O are float32; the weights are rounded to the
 // operands' type for P V, which makes the result's error 1.4 times that of its own rounding.
@@ -36,6 +38,8 @@
 // 123 us. One query over 32640 keys, 2 x 16 heads of 64: 68 us (3.9 TB/s), where what is left
 // is the start, the pieces and their join.
 #pragma once
+#include <cfloat>
+
 #include "op_attn.cuh"
 
 namespace scb {
@@ -44,6 +48,7 @@ constexpr int AT_KEYS = 128;               // keys of a tile
 constexpr int AT_THREADS = 640;
 constexpr int AT_REGS = 96;                // registers a thread at launch (checked there)
 constexpr float AT_STALE = 8.f;            // log2 by which a tile may exceed m
+constexpr float AT_LOWEST = -FLT_MAX;      // m of visible scores that are all -inf
 constexpr int AT_BOX = AT_KEYS * 128;      // bytes of 128 rows x 64 channels
 
 // Of every 16 pairs of weights, those whose 2^y is computed by exp2_pair on the FMA units
@@ -130,6 +135,11 @@ __device__ __forceinline__ float2 exp2_pair(float2 y) {
       : "r"(__float_as_int(z.y)), "r"(kZero ? 127 << 23 : __float_as_int(p.y)));
   const float2 r = make_float2(__int_as_float(rx), __int_as_float(ry));
   return kZero ? __fmul2_rn(p, r) : r;
+}
+
+// 1 / l of a row's final sum: 0 when no key was visible, NaN when nothing was above -inf.
+__device__ __forceinline__ float at_inverse(float m, float l) {
+  return m == -INFINITY && l == l ? 0.f : l >= 0.5f ? 1.f / l : NAN;
 }
 
 // A sum of weights as it is, or NaN when a weight was (weights are at most 2^8, so a sum of
@@ -506,7 +516,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             fence_proxy_async_smem();
           }
         }
-        float top = live ? row_max<64>(s) : -INFINITY;
+        // (-inf only where this half's 64 keys are all hidden)
+        float top = part && !(seen[0] | seen[1]) ? -INFINITY : live ? fmaxf(row_max<64>(s), AT_LOWEST) : AT_LOWEST;
         if (cnt > first) at_wait(o_done + t, (cnt - 1) & 1, dead, AT_O);  // O_t is complete, P_t read
         // (the barrier also keeps P_t, where it lies over S_t, behind both halves' loads)
         if (at_any(id, j == jt || top > m + stale)) {
@@ -531,7 +542,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           }
         }
         // an infinite score makes the row NaN, as inf - inf would
-        const float mc = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m * c;
+        const float mc = m <= AT_LOWEST ? 0.f : m == INFINITY ? NAN : -m * c;
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if (!Twin || g.turns) at_turn_wait(t);
 #pragma unroll
@@ -580,7 +591,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       if (!Twin && n == g.tiles) {
         // through the Q tile, whose products are complete: 16-byte chunks of whole rows,
         // `wide` lanes a row, as Q was read
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = at_inverse(m, l);
         for (int i = half; live && i < ksteps; i += 2) {
           float v[16];
           tmem_ld16(to + 16 * i, v);
@@ -610,7 +621,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         // the piece is kept channel by channel, so that a warp stores 32 rows side by side
         const long piece = 2L * blockIdx.x + (x == x0 ? 0 : 1);
         const int col = Twin ? 128 * t + unit_row : unit_row;
-        if (half == 0) g.part_ml[piece * 256 + col] = make_float2(m == -INFINITY ? m : m * c, l);
+        if (half == 0) g.part_ml[piece * 256 + col] = make_float2(m == -INFINITY ? m : fmaxf(m * c, AT_LOWEST), l);
         float* o = g.part + piece * 256 * d + col;
         for (int i = half; live && i < ksteps; i += 2) {
           float v[16];
@@ -635,8 +646,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 
 // Adds the pieces of the units that were cut, 32 rows a block:
 //   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, M the largest m_i
-// A piece without a score for a row (m_i = -inf) weighs nothing, but a NaN in its total, that
-// of a NaN score (maxima skip those), makes the row NaN as it does in an uncut unit.
+// A piece without a visible key for a row (m_i = -inf) weighs nothing; a NaN in any piece's
+// total makes the row NaN as it does in an uncut unit.
 // A lane is a row (the pieces are stored channel by channel). All maxima and totals are
 // fetched at once and turned into weights in shared memory, then every warp adds its
 // channels, whose loads wait for nothing (piece by piece, each behind its maximum, took 15 to
@@ -697,7 +708,7 @@ __global__ void __launch_bounds__(AT_JOIN) attn_join_kernel(const __grid_constan
         o[k] += f == 0.f ? 0.f : f * v;
       }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = at_inverse(top, l);
 #pragma unroll
   for (int k = 0; k < kMost; ++k)
     if (warp + k * kWarps < d) out[lane][warp + k * kWarps] = from_f32<T>(o[k] * inv);

@@ -19,6 +19,26 @@ def infinite_keys(torch, cut, dt, seed):  # noqa: F811
 
 @cuts
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_all_visible_scores_minus_infinity(torch, ops, cut, dtype):  # noqa: F811
+    """softmax of nothing but -inf is 0 / 0: NaN, with and without hidden keys beside them; with
+    no visible key the row is zero, whatever the hidden keys score."""
+    q, k, v = infinite_keys(torch, cut, getattr(torch, dtype), 61)
+    ordinary = k.clone()
+    k[0, :, :, 0] = -math.inf
+    out = ops.attention(q, k, v)
+    assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
+    mask = torch.zeros(k.shape[:2], dtype=torch.bool, device="cuda")
+    mask[:, 3] = mask[:, -2] = True
+    out = ops.attention(q, k, v, key_mask=mask)
+    assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
+    mask[0] = False
+    out = ops.attention(q, k, v, key_mask=mask)
+    assert not out[0].any()
+    check_attention(torch, ops, q, ordinary, v, mask, got=out)
+
+
+@cuts
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("finite", ["first", "last", "some"])
 def test_some_scores_minus_infinity(torch, ops, cut, dtype, finite):  # noqa: F811
     """Such keys weigh nothing where a row has a finite score, as hidden keys do."""
@@ -32,6 +52,14 @@ def test_some_scores_minus_infinity(torch, ops, cut, dtype, finite):  # noqa: F8
     bad = torch.where(keep[:, :, None, None], k, torch.tensor(-math.inf, device="cuda", dtype=k.dtype))
     bad[..., 1:] = k[..., 1:]
     check_attention(torch, ops, q, k, v, keep, got=ops.attention(q, bad, v))
+
+
+@cuts
+def test_bf16_products_that_overflow(torch, ops, cut):  # noqa: F811
+    """Finite operands whose scores overflow to -inf, in every row."""
+    q, k, v = infinite_keys(torch, cut, torch.bfloat16, 63)
+    q[..., 0], k[..., 0] = 1e30, -1e30
+    assert torch.isnan(ops.attention(q, k, v)).all()
 
 
 @cuts
