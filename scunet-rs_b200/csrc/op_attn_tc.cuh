@@ -16,14 +16,14 @@
 // K and V into a ring of 128-key slots (warp 19 fills the warpgroup up, which gives
 // registers to the softmax).
 //   S_t = Q_t K^T    M 128, N 128, K d        TMEM columns [128 t, +128)
-//   P_t = 2^(c S - c m), 16-bit               64 columns
+//   P_t = 2^(c S - c m + AT_LIFT), 16-bit     64 columns
 //   O_t += P_t V     M 128, N d, K 128        columns [256 + 64 or 128 t, +d), A from TMEM
 // Heads up to 64 wide leave columns for P_t beside S_t, and wider ones keep P_t in shared
 // memory, so the next S_t is computed as soon as this one is in registers (Twin with wide
 // heads: P_t lies over S_t, and the next S_t waits for P_t V). While one tile's softmax
 // runs, the tensor cores compute the other tile's products. The maximum m that a row
 // subtracts is raised only when a tile exceeds it by 2^8 (in P): sums are float32 and P at
-// most 256, so a stale m changes no result, and O, which lives in TMEM, is rescaled only
+// most 256 (2^15 with AT_LIFT), so a stale m changes no result, and O, which lives in TMEM, is rescaled only
 // then. m is -inf while no key was visible and at least AT_LOWEST after that, so the end can
 // tell rows that see nothing (zeros) from rows whose visible scores are all -inf (0 / 0, NaN):
 // the weights of any other row sum up to 1 or more.
@@ -48,6 +48,11 @@ constexpr int AT_KEYS = 128;               // keys of a tile
 constexpr int AT_THREADS = 640;
 constexpr int AT_REGS = 96;                // registers a thread at launch (checked there)
 constexpr float AT_STALE = 8.f;            // log2 by which a tile may exceed m
+// log2 by which weights (and so their sums and O) are kept larger than 2^(c S - c m): 2^15 at
+// most with AT_STALE. fp16 loses what is below 2^-25, which a long faint tail would show: this
+// way that is 2^-32 of the row's largest weight, 2^-32 times the keys in all.
+template <typename T>
+constexpr float AT_LIFT = __is_same(T, __half) ? 7.f : 0.f;
 constexpr float AT_LOWEST = -FLT_MAX;      // m of visible scores that are all -inf
 constexpr int AT_BOX = AT_KEYS * 128;      // bytes of 128 rows x 64 channels
 
@@ -105,7 +110,7 @@ __device__ __forceinline__ uint32_t at_pack<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// 2^y of two values y <= 8 on the FMA units: y = n + f, n the nearest integer (it appears in
+// 2^y of two values y <= 15 on the FMA units: y = n + f, n the nearest integer (it appears in
 // the low bits of y + 1.5 2^23), |f| <= 1/2; 2^f by the cubic of least relative error on that
 // interval (fitted by linear programming: 7.5e-5 at most, 5.2e-5 rms, where rounding the
 // weight to fp16 adds 2e-4 rms and to bf16 1.6e-3). For fp16 n is added to the exponent: y
@@ -142,7 +147,7 @@ __device__ __forceinline__ float at_inverse(float m, float l) {
   return m == -INFINITY && l == l ? 0.f : l >= 0.5f ? 1.f / l : NAN;
 }
 
-// A sum of weights as it is, or NaN when a weight was (weights are at most 2^8, so a sum of
+// A sum of weights as it is, or NaN when a weight was (weights are at most 2^15, so a sum of
 // them stays far below 1e30).
 __device__ __forceinline__ float at_total(float l) { return l < 1e30f ? l : NAN; }
 
@@ -541,8 +546,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             }
           }
         }
-        // an infinite score makes the row NaN, as inf - inf would
-        const float mc = m <= AT_LOWEST ? 0.f : m == INFINITY ? NAN : -m * c;
+        // (a score of +inf makes m infinite, its own weight inf - inf, and the row's total, NaN)
+        const float mc = m <= AT_LOWEST ? 0.f : fmaf(-m, c, AT_LIFT<T>);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         if (!Twin || g.turns) at_turn_wait(t);
 #pragma unroll
