@@ -305,6 +305,6 @@ class RotateAxes(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
-        dq, dk = rotate_axes(dq.contiguous(), dk.contiguous(), positions, inv_freq, ctx.sections, layout=ctx.layout,
-                             inverse=True)
+        dk = None if dk is None else dk.contiguous()  # there was no k
+        dq, dk = rotate_axes(dq.contiguous(), dk, positions, inv_freq, ctx.sections, layout=ctx.layout, inverse=True)
         return dq, dk, None, None, None, None
