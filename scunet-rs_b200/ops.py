@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .backend import (SCB_ACTS, SCB_BF16, SCB_F16, SCB_F32, SCB_I32, SCB_I64, SCB_ROT_LAYOUTS, BackendError, ScbHeads,
                       ScbRows, load_library)
@@ -276,7 +277,8 @@ def status(stream=None):
 
 
 class GroupNormAct(torch.autograd.Function):
-    """group_norm under autograd: GroupNormAct.apply(x, groups, weight, bias, eps, act)."""
+    """group_norm under autograd: GroupNormAct.apply(x, groups, weight, bias, eps, act). It has
+    no second derivative: differentiating its gradient raises RuntimeError."""
 
     @staticmethod
     def forward(ctx, x, groups, weight, bias, eps=1e-5, act="none"):
@@ -286,6 +288,7 @@ class GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, mean, rstd, weight, bias = ctx.saved_tensors
         dy = dy.contiguous()  # a gradient may come broadcast
@@ -294,17 +297,19 @@ class GroupNormAct(torch.autograd.Function):
 
 
 class RotateAxes(torch.autograd.Function):
-    """rotate_axes under autograd: RotateAxes.apply(q, k, positions, inv_freq, sections, layout)."""
+    """rotate_axes under autograd: RotateAxes.apply(q, k, positions, inv_freq, sections, layout,
+    inverse). Its gradient is the rotation by the opposite angles, under autograd again, so it
+    has derivatives of every order."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, sections, layout="half"):
+    def forward(ctx, q, k, positions, inv_freq, sections, layout="half", inverse=False):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.sections, ctx.layout = tuple(sections), layout
-        return rotate_axes(q, k, positions, inv_freq, sections, layout=layout)
+        ctx.sections, ctx.layout, ctx.inverse = tuple(sections), layout, bool(inverse)
+        return rotate_axes(q, k, positions, inv_freq, sections, layout=layout, inverse=inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         dk = None if dk is None else dk.contiguous()  # there was no k
-        dq, dk = rotate_axes(dq.contiguous(), dk, positions, inv_freq, ctx.sections, layout=ctx.layout, inverse=True)
-        return dq, dk, None, None, None, None
+        dq, dk = RotateAxes.apply(dq.contiguous(), dk, positions, inv_freq, ctx.sections, ctx.layout, not ctx.inverse)
+        return dq, dk, None, None, None, None, None

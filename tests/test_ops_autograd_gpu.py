@@ -20,3 +20,47 @@ def test_rotate_axes_without_k(torch, ops):  # noqa: F811
     y.backward(dy)
     want = rotate64(torch, dy, pos, freq, (7, 7), "axial", True)
     within(q.grad, want, 8 * E * dy.double().abs().amax(-1, keepdim=True) + E * want.abs(), "dq")
+
+
+def test_group_norm_has_no_second_derivative(torch, ops):  # noqa: F811
+    """A gradient penalty needs it: an error, not a wrong gradient."""
+    x = torch.randn((2, 40, 32), generator=gen(torch, 82), device="cuda").requires_grad_()
+    w = torch.ones(32, device="cuda", requires_grad=True)
+    y = ops.GroupNormAct.apply(x, 4, w, None, 1e-5, "silu")
+    dx, = torch.autograd.grad((y * x).sum(), x, create_graph=True)  # x also reaches the loss directly
+    with pytest.raises(RuntimeError, match="differentiat"):
+        dx.square().sum().backward()
+    # without create_graph all is as before
+    dx, = torch.autograd.grad(ops.GroupNormAct.apply(x, 4, w, None, 1e-5, "silu").square().sum(), x)
+    assert torch.isfinite(dx).all() and not dx.requires_grad
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved", "axial"])
+def test_rotate_axes_second_derivative(torch, ops, layout):  # noqa: F811
+    """The rotation is linear, its gradient is the inverse rotation, and so on."""
+    pos, freq = positions(torch)
+    q, k = (torch.randn((2, 31, n, 32), generator=gen(torch, 83 + n), device="cuda") for n in (4, 2))
+
+    def penalty(turn, q, k):
+        yq, yk = turn(q, k)
+        dq, dk = torch.autograd.grad((yq ** 3).sum() + (yk ** 3).sum() + (q ** 2).sum(), (q, k), create_graph=True)
+        return torch.autograd.grad(dq.square().sum() + (dk ** 2).sum(), (q, k))
+
+    def plain(q, k):
+        return tuple(rotate64(torch, t, pos, freq, (7, 7), layout, False) for t in (q, k))
+
+    got = penalty(lambda a, b: ops.RotateAxes.apply(a, b, pos, freq, (7, 7), layout),
+                  q.clone().requires_grad_(), k.clone().requires_grad_())
+    want = penalty(plain, q.double().requires_grad_(), k.double().requires_grad_())
+    for a, b in zip(got, want):  # a chain of four rotations and some powers: below 100 operations on the row's terms
+        within(a, b, 100 * E * (1 + b.abs().amax((2, 3), keepdim=True)), layout)
+
+
+def test_rotate_axes_inverse_under_autograd(torch, ops):  # noqa: F811
+    pos, freq = positions(torch)
+    q = torch.randn((2, 31, 4, 32), generator=gen(torch, 86), device="cuda").requires_grad_()
+    there = ops.RotateAxes.apply(q, None, pos, freq, (7, 7))[0]
+    back = ops.RotateAxes.apply(there, None, pos, freq, (7, 7), "half", True)[0]
+    g = torch.randn_like(q)
+    back.backward(g)
+    within(q.grad, g.double(), 16 * E * g.double().abs().amax(-1, keepdim=True), "identity's gradient")
