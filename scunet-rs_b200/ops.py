@@ -9,7 +9,9 @@
 Every call runs on the current stream of its tensors' device, takes its outputs and its
 workspace from torch's caching allocator (so a workspace lives as long as the stream needs
 it) and returns before the GPU has finished. Inputs may be views: only the channels have to
-be contiguous. `GroupNormAct` and `RotateAxes` are the same for autograd. Wrong arguments
+be contiguous; an `out` may not overlap an input except where that is said. `GroupNormAct`
+and `RotateAxes` are the same for autograd; the functions themselves, and attention, which has
+no gradient, refuse tensors that require one while gradients are recorded. Wrong arguments
 raise `BackendError`; there is no fallback for tensors that are not on a CUDA device.
 """
 from __future__ import annotations
@@ -98,6 +100,17 @@ def _params(t, c, like, what):
     return t.data_ptr()
 
 
+_recording = torch.is_grad_enabled
+
+
+def _no_gradient(why, *tensors):
+    """Refuses tensors whose gradient the call would drop from the graph without a word (the
+    caller has looked whether gradients are recorded at all)."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            _fail(why + " (or call it under torch.no_grad())")
+
+
 def _rows(t, what):
     """(pictures, rows, channels, picture stride, row stride) of [n][...][c]; the dimensions
     between collapse to rows of one stride."""
@@ -146,6 +159,8 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act="none", out=N
     and bias are float32 [c]; act is "none", "relu", "gelu" (exact) or "silu". `out` may be x.
     With stats=True also returns mean and 1 / sqrt(var + eps), float32 [n, groups]."""
     dt = _dtype(x, "x")
+    if _recording():
+        _no_gradient("group_norm gives no gradient: use GroupNormAct.apply", x, weight, bias, out)
     n, l, c, sn, sl = _rows(x, "x")
     y = _out(out, x)
     yn, yl = (l * c, c) if out is None else _rows(y, "out")[3:]
@@ -163,6 +178,8 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, ac
     dweight and dbias are float32 [c] whether or not weight and bias are given; `out` (dx) may
     be dy or x."""
     dt = _dtype(x, "x")
+    if _recording():
+        _no_gradient("group_norm has no second derivative", dy, x, mean, rstd, weight, bias, out)
     n, l, c, sn, sl = _rows(x, "x")
     _same(dy, x, "dy")
     _, _, _, dn, dl = _rows(dy, "dy")
@@ -186,6 +203,9 @@ def _sections(sections):
     return (ctypes.c_int * len(sections))(*sections), sum(sections)
 
 
+_NO_POSITIONS = "the rotation has no gradient with respect to positions and inv_freq"
+
+
 def _heads(x, out, what):
     if x.dim() != 4:
         _fail(f"{what} must be [pictures, tokens, heads, channels]")
@@ -206,6 +226,10 @@ def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=F
     copied. inverse=True turns back, which is the gradient. `out` is a pair of tensors, which
     may be (q, k) themselves."""
     dt = _dtype(q, "q")
+    if _recording():
+        _no_gradient("rotate_axes gives no gradient: use RotateAxes.apply", q, k, *(out or ()))
+        if positions.requires_grad or inv_freq.requires_grad:
+            _fail(_NO_POSITIONS)
     if layout not in SCB_ROT_LAYOUTS:
         _fail(f"unknown layout {layout!r}")
     if q.dim() != 4:
@@ -239,8 +263,10 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
     q is [b, lq, h, d], k and v [b, lk, hk, d] with d at most 256; query head i reads key head
     i / (h / hk). key_mask is bool or uint8 [b, lk], nonzero = visible: what hidden keys hold
     does not matter, and queries with no visible key give zeros. scale defaults to
-    1 / sqrt(d). Fast (tensor cores) for d up to 128 and 16-byte aligned rows of k and v."""
+    1 / sqrt(d). Forward only: there is no gradient. Fast (tensor cores) for d up to 128 and 16-byte aligned rows of k and v."""
     dt = _dtype(q, "q")
+    if _recording():
+        _no_gradient("attention has no gradient", q, k, v, out)
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         if t.dim() != 4 or t.dtype != q.dtype or t.get_device() != q.get_device():
             _fail(f"{what} must be [pictures, tokens, heads, channels] {q.dtype} on {q.device}")
@@ -310,6 +336,8 @@ class RotateAxes(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+            _fail(_NO_POSITIONS)
         dk = None if dk is None else dk.contiguous()  # there was no k
         dq, dk = RotateAxes.apply(dq.contiguous(), dk, positions, inv_freq, ctx.sections, ctx.layout, not ctx.inverse)
         return dq, dk, None, None, None, None, None

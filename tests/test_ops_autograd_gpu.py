@@ -1,7 +1,7 @@
 """The block operators and autograd."""
 import pytest
 
-from test_ops_gpu import E, gen, ops, rotate64, torch, within  # noqa: F401 (fixtures)
+from test_ops_gpu import E, gen, ops, qkv_of, rotate64, torch, within  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,45 @@ def test_rotate_axes_inverse_under_autograd(torch, ops):  # noqa: F811
     g = torch.randn_like(q)
     back.backward(g)
     within(q.grad, g.double(), 16 * E * g.double().abs().amax(-1, keepdim=True), "identity's gradient")
+
+
+def test_gradients_that_would_be_lost_are_refused(torch, ops, scb):  # noqa: F811
+    pos, freq = positions(torch)
+    x = torch.randn((2, 31, 4, 32), generator=gen(torch, 87), device="cuda")
+    w = torch.ones(32, device="cuda")
+    m = torch.ones((2, 4), device="cuda")
+    q, k, v = qkv_of(torch, 1, 40, 50, 2, 2, 64, torch.float16)
+
+    def on(t):
+        return t.clone().requires_grad_()
+
+    calls = {
+        "GroupNormAct": [lambda: ops.group_norm(on(x), 4), lambda: ops.group_norm(x, 4, on(w)),
+                         lambda: ops.group_norm(x, 4, None, on(w)), lambda: ops.group_norm(x, 4, out=on(x))],
+        "second": [lambda: ops.group_norm_backward(on(x), x, m, m, 4), lambda: ops.group_norm_backward(x, on(x), m, m, 4),
+                   lambda: ops.group_norm_backward(x, x, on(m), m, 4), lambda: ops.group_norm_backward(x, x, m, on(m), 4),
+                   lambda: ops.group_norm_backward(x, x, m, m, 4, on(w))],
+        "RotateAxes": [lambda: ops.rotate_axes(on(x), None, pos, freq, (7, 7)),
+                       lambda: ops.rotate_axes(x, on(x), pos, freq, (7, 7)),
+                       lambda: ops.rotate_axes(x, x, pos, freq, (7, 7), out=(x.clone(), on(x)))],
+        "inv_freq": [lambda: ops.rotate_axes(x, None, pos.float().requires_grad_(), freq, (7, 7)),
+                     lambda: ops.rotate_axes(x, None, pos, on(freq), (7, 7))],
+        "attention": [lambda: ops.attention(on(q), k, v), lambda: ops.attention(q, on(k), v),
+                      lambda: ops.attention(q, k, on(v)), lambda: ops.attention(q, k, v, out=on(q))],
+    }
+    for words, some in calls.items():
+        for call in some:
+            with pytest.raises(scb.BackendError, match=words):
+                call()
+    with torch.no_grad():  # nobody asks for a gradient: they run
+        for some in calls.values():
+            for call in some:
+                call()
+    with torch.inference_mode():
+        ops.attention(q, k, v, out=torch.empty_like(q))
+    for turn in (lambda: ops.RotateAxes.apply(x, None, pos, on(freq), (7, 7)),
+                 lambda: ops.RotateAxes.apply(on(x), x, pos.float().requires_grad_(), freq, (7, 7))):
+        with pytest.raises(scb.BackendError, match="inv_freq"):
+            turn()[0].sum().backward()
+        with torch.no_grad():
+            turn()
