@@ -9,10 +9,11 @@
 Every call runs on the current stream of its tensors' device, takes its outputs and its
 workspace from torch's caching allocator (so a workspace lives as long as the stream needs
 it) and returns before the GPU has finished. Inputs may be views: only the channels have to
-be contiguous; an `out` may not overlap an input except where that is said. `GroupNormAct`
-and `RotateAxes` are the same for autograd; the functions themselves, and attention, which has
-no gradient, refuse tensors that require one while gradients are recorded. Wrong arguments
-raise `BackendError`; there is no fallback for tensors that are not on a CUDA device.
+be contiguous. An `out` may not overlap an input except where that is said, and counts as
+written in place for autograd. `GroupNormAct` and `RotateAxes` are the same for autograd; the
+functions themselves, and attention, which has no gradient, refuse tensors that require one
+while gradients are recorded. Wrong arguments raise `BackendError`; there is no fallback for
+tensors that are not on a CUDA device.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ import functools
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from .backend import (SCB_ACTS, SCB_BF16, SCB_F16, SCB_F32, SCB_I32, SCB_I64, SCB_ROT_LAYOUTS, BackendError, ScbHeads,
                       ScbRows, load_library)
@@ -170,6 +172,8 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act="none", out=N
     _work, work, size = _workspace("scb_group_norm_workspace", x, n, l, c, groups)
     _call(x, _library().scb_group_norm, x.data_ptr(), sn, sl, dt, n, l, c, groups, _params(weight, c, x, "weight"),
           _params(bias, c, x, "bias"), eps, _act(act), y.data_ptr(), yn, yl, _ptr(mean), _ptr(rstd), work, size)
+    if out is not None:
+        increment_version(out)
     return (y, mean, rstd) if stats else y
 
 
@@ -194,6 +198,8 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, *, ac
     _call(x, _library().scb_group_norm_backward, dy.data_ptr(), dn, dl, x.data_ptr(), sn, sl, dt, n, l, c, groups,
           mean.data_ptr(), rstd.data_ptr(), _params(weight, c, x, "weight"), _params(bias, c, x, "bias"), _act(act),
           dx.data_ptr(), xn, xl, dw.data_ptr(), db.data_ptr(), work, size)
+    if out is not None:
+        increment_version(out)
     return dx, dw, db
 
 
@@ -254,6 +260,9 @@ def rotate_axes(q, k, positions, inv_freq, sections, *, layout="half", inverse=F
     _call(q, _library().scb_rotate_axes, _heads(q, yq, "q"), None if k is None else _heads(k, yk, "k"), dt, b, l, d,
           positions.data_ptr(), _POSITIONS[positions.dtype], pb, pl, pa, inv_freq.data_ptr(),
           c_sections, axes, SCB_ROT_LAYOUTS[layout], bool(inverse))
+    if out is not None:
+        for y in (yq,) if k is None else (yq, yk):
+            increment_version(y)
     return yq, yk
 
 
@@ -290,6 +299,8 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
     _work, work, size = _workspace("scb_attention_workspace", q, b, lq, lk, h, hk, d)
     _call(q, _library().scb_attention, *rows, dt, b, lq, lk, h, hk, d, _ptr(key_mask),
           0 if key_mask is None else key_mask.stride(0), d ** -0.5 if scale is None else scale, work, size)
+    if out is not None:
+        increment_version(out)
     return o
 
 

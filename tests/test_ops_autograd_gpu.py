@@ -106,3 +106,25 @@ def test_gradients_that_would_be_lost_are_refused(torch, ops, scb):  # noqa: F81
             turn()[0].sum().backward()
         with torch.no_grad():
             turn()
+
+
+def test_out_counts_as_written(torch, ops):  # noqa: F811
+    """Writing over a tensor that autograd saved is found in the backward pass."""
+    pos, freq = positions(torch)
+    x = torch.randn((2, 31, 4, 32), generator=gen(torch, 88), device="cuda")
+    stats = ops.group_norm(x, 4, stats=True)[1:]
+    q, k, v = qkv_of(torch, 1, 40, 50, 2, 2, 64, torch.float16)
+    writes = [
+        (x, lambda t: ops.group_norm(x, 4, out=t)),
+        (x, lambda t: ops.group_norm_backward(x, x, *stats, 4, out=t)),
+        (x, lambda t: ops.rotate_axes(x, None, pos, freq, (7, 7), out=(t, None))),
+        (x, lambda t: ops.rotate_axes(x, x, pos, freq, (7, 7), out=(torch.empty_like(x), t))),
+        (q, lambda t: ops.attention(q, k, v, out=t)),
+    ]
+    for like, write in writes:
+        w = torch.ones_like(like, requires_grad=True)
+        saved = like.clone()
+        y = (w * saved).sum()
+        write(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
