@@ -27,7 +27,10 @@
 //
 // Statistics are fp32: a block sums x - K and (x - K)^2 with K the median of the channel's
 // values in its first, middle and last row, so that the sum of squares loses nothing to a
-// large mean or to one value far from the rest, and (count, mean, M2) triples are joined,
+// large mean or to one value far from the rest. Two of those three rows may be far from the
+// rest, as where a map has a border of its own: a block whose K lies more than eight spreads
+// from its mean (NORM_FAR) sums once more, about that mean (rstd 2.5e-3 off before, 1e6 at both
+// ends of 1088 x 1920 rows). (count, mean, M2) triples are joined,
 //   M2 = M2a + M2b + (mb - ma)^2 na nb / (na + nb).
 // No atomics: the order of every sum is fixed by the sizes.
 #pragma once
@@ -56,6 +59,8 @@ struct NormGeom {
 };
 
 constexpr int NORM_THREADS = 512;  // two blocks an SM: every block reads its picture's partials
+
+constexpr float NORM_FAR = 64.f;   // of a group: sum of (x - K)^2 over M2 that a block accepts
 
 // Blocks of the gradient an SM: vectors of 8 take more than the 64 registers that two leave.
 __host__ __device__ constexpr int norm_grad_blocks(int vec) { return vec == 8 ? 1 : 2; }
@@ -279,22 +284,36 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // Mean and M2 of channels [lo, hi) of a chunk over `rows` rows, by one warp: the channels'
-// means average to the group's, M2 = sum (M2_c + rows (mean_c - mean)^2).
+// means average to the group's, M2 = sum (M2_c + rows (mean_c - mean)^2). `far` is set where
+// the sums about `first` lose too much of M2.
 template <int V, int T>
 __device__ __forceinline__ float2 group_moments(const BlockSums<V, T>& s, const float* first, int lo, int hi,
-                                                float rows) {
+                                                float rows, bool& far) {
   const int lane = threadIdx.x & 31;
   const float inv = rows > 0.f ? 1.f / rows : 0.f;
   float mean = 0.f;
   for (int ch = lo + lane; ch < hi; ch += 32) mean += first[ch] + s.at(ch).x * inv;
   mean = warp_sum(mean) / (float)(hi - lo);
-  float m2 = 0.f;
+  float m2 = 0.f, sq = 0.f;
   for (int ch = lo + lane; ch < hi; ch += 32) {
     const float2 v = s.at(ch);
     const float d = first[ch] + v.x * inv - mean, own = v.y - v.x * v.x * inv;
     m2 += (own < 0.f ? 0.f : own) + rows * d * d;  // (a NaN stays)
+    sq += v.y;
   }
-  return make_float2(mean, warp_sum(m2));
+  m2 = warp_sum(m2);
+  far = far || warp_sum(sq) > NORM_FAR * m2;
+  return make_float2(mean, m2);
+}
+
+// Whether any thread of the block found a group's sums too far off; then K of the chunk's
+// channels becomes their mean.
+template <int V, int T>
+__device__ __forceinline__ bool recentre(const BlockSums<V, T>& s, float* first, float rows, bool far) {
+  if (!__syncthreads_or(far)) return false;
+  for (int ch = threadIdx.x; ch < s.channels; ch += T) first[ch] += s.at(ch).x / rows;
+  __syncthreads();
+  return true;
 }
 
 // The channels' K from `many` rows, `stride` elements apart.
@@ -443,6 +462,47 @@ struct NormPlace {
   }
 };
 
+// A block's sums about `first` joined to the mean and M2 of its part of every group of its chunk;
+// whether `first` is too far from the means (in some thread).
+template <int V>
+__device__ __forceinline__ bool norm_partials(const NormGeom& g, const NormPlace& p,
+                                              const BlockSums<V, NORM_THREADS>& sums, const float* first,
+                                              float2* part) {
+  bool far = false;
+  float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
+  for (int grp = p.c0 / g.cpg + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
+    const float2 m = group_moments(sums, first, max(grp * g.cpg, p.c0) - p.c0, min((grp + 1) * g.cpg, p.c1) - p.c0,
+                                   norm_rows(g, p.split), far);
+    if ((threadIdx.x & 31) == 0) out[grp] = m;
+  }
+  return far;
+}
+
+// The block's sums once more, about `first`, for which it has moved. (Rare, and a function of its
+// own, so that it takes no registers from the first time, which would spill.)
+template <typename T, int V>
+__device__ __noinline__ void norm_stats_again(const T* x, float2* part, const NormGeom& g, float* mem) {
+  const NormPlace p(g, V);
+  const float* first = mem + g.keep;
+  float k[V], sum[V], sq[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    k[i] = first[(threadIdx.x - p.lane * g.tc) * V + i];
+    sum[i] = sq[i] = 0.f;
+  }
+  const T* src = x + p.pic * g.x_sn + p.first * g.x_sl + (long)p.col * V;
+  for (long n = p.mine(g); n > 0; --n, src += p.step * g.x_sl) {
+    Pack<T, V> a;
+    float v[V];
+    a.load(src);
+    unpack(a, v);
+    add_moments<V>(v, k, sum, sq);
+  }
+  BlockSums<V, NORM_THREADS> sums;
+  sums.add(mem, g, sum, sq, p.lane);
+  norm_partials<V>(g, p, sums, first, part);
+}
+
 // First pass: per (picture, split, chunk's part of a group) mean and M2.
 template <typename T, int V>
 __global__ void __launch_bounds__(NORM_THREADS, 2)
@@ -485,12 +545,8 @@ norm_stats_kernel(const T* __restrict__ x, float2* __restrict__ part, const __gr
   __syncthreads();  // the sums lie over the ring
   BlockSums<V, NORM_THREADS> sums;
   sums.add(norm_sm, g, sum, sq, p.lane);
-  float2* out = part + (p.pic * g.splits + p.split) * g.slots + p.chunk;
-  for (int grp = p.c0 / g.cpg + (threadIdx.x >> 5); grp * g.cpg < p.c1; grp += NORM_THREADS / 32) {
-    const float2 m = group_moments(sums, first, max(grp * g.cpg, p.c0) - p.c0, min((grp + 1) * g.cpg, p.c1) - p.c0,
-                                   norm_rows(g, p.split));
-    if ((threadIdx.x & 31) == 0) out[grp] = m;
-  }
+  const bool far = norm_partials<V>(g, p, sums, first, part);
+  if (recentre(sums, first, norm_rows(g, p.split), far)) norm_stats_again<T, V>(x, part, g, norm_sm);
 }
 
 // Partials s0, s0 + 32, ... of a picture's slot, all on their way at once.
@@ -833,10 +889,24 @@ norm_small_kernel(const T* dy, const T* x, T* y, float* __restrict__ mean,
       for (int i = 0; i < V; ++i) first[t * V + i] = k[i];
     }
     BlockSums<V, kT> sums;
-    sums.add(norm_sm, g, sum, sq, p.lane);
-    for (int n = threadIdx.x >> 5; n < ng; n += kT / 32) {
-      const float2 m = group_moments(sums, first, n * g.cpg, (n + 1) * g.cpg, (float)rows);
-      if ((threadIdx.x & 31) == 0) share[n] = m;
+    for (bool again = false;; again = true) {  // twice where K turns out to be far from the mean
+      sums.add(norm_sm, g, sum, sq, p.lane);
+      bool far = false;
+      for (int n = threadIdx.x >> 5; n < ng; n += kT / 32) {
+        const float2 m = group_moments(sums, first, n * g.cpg, (n + 1) * g.cpg, (float)rows, far);
+        if ((threadIdx.x & 31) == 0) share[n] = m;
+      }
+      if (again || !recentre(sums, first, (float)rows, far)) break;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        k[i] = first[t * V + i];
+        sum[i] = sq[i] = 0.f;
+      }
+      for (long row = p.on ? p.lane : rows; row < rows; row += g.rp) {
+        float v[V];
+        unpack(keep[row * g.tc + t], v);
+        add_moments<V>(v, k, sum, sq);
+      }
     }
     g.splits > 1 ? cluster_sync() : __syncthreads();
     for (int n = threadIdx.x; n < ng; n += kT) {
