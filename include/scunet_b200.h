@@ -311,7 +311,8 @@ int scb_profile_report(scb_ctx* ctx, char* buf, size_t cap);
  * by one call at a time) and a stream (NULL: the default stream). They are asynchronous,
  * allocate nothing and can be captured in a CUDA graph. Inputs may overlap one another
  * (stride 0 broadcasts), outputs may not, except as stated. On failure the message is in
- * scb_last_error (NULL) of the calling thread, and nothing was launched.
+ * scb_last_error (NULL) of the calling thread; a refused argument launches nothing, and after
+ * a failed launch the outputs are undefined.
  * ------------------------------------------------------------------------------------- */
 enum { SCB_ACT_NONE = 0, SCB_ACT_RELU = 1, SCB_ACT_GELU = 2, SCB_ACT_SILU = 3 };
 

@@ -25,10 +25,12 @@ namespace {
 
 int refuse(const char* op, const std::string& msg) { return global_error(SCB_EINVAL, std::string(op) + ": " + msg); }
 
-int launched(const char* op) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string(op) + ": " + cudaGetErrorString(e));
-  return SCB_OK;
+// What the runtime calls and launches of an operator came to. A failure is taken back from the
+// runtime's memory of it, or the next call would report it as its own.
+int finished(const char* op, cudaError_t e) {
+  if (e == cudaSuccess) return SCB_OK;
+  cudaGetLastError();
+  return global_error(SCB_ECUDA, std::string(op) + ": " + cudaGetErrorString(e));
 }
 
 // No C++ exception leaves a C entry (std::string may fail to allocate).
@@ -37,7 +39,11 @@ int guarded(F&& f) noexcept {
   try {
     return f();
   } catch (...) {
-    return SCB_ENOMEM;
+    try {
+      return global_error(SCB_ENOMEM, "out of memory");  // short enough to need none
+    } catch (...) {
+      return SCB_ENOMEM;
+    }
   }
 }
 
@@ -47,26 +53,39 @@ uint64_t addr(const void* p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); 
 
 int sm_count() {
   int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return sms;
+  if (cudaGetDevice(&dev) == cudaSuccess &&
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+    return sms;
+  cudaGetLastError();
+  return 0;
 }
 
-// Launch `kernel` so that it may start while the launch before it in the stream ends
-// (it waits for that launch's results itself).
+// A launch, which returns its own error (cudaGetLastError after it would return one that was
+// left from before). `with`: one attribute, or null.
 template <typename... P, typename... A>
-void launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+cudaError_t launch_with(cudaLaunchAttribute* with, void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                        cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  a[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = a;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  cfg.attrs = with;
+  cfg.numAttrs = with ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  return launch_with(nullptr, kernel, grid, threads, smem, st, args...);
+}
+// Launch `kernel` so that it may start while the launch before it in the stream ends
+// (it waits for that launch's results itself).
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute a;
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return launch_with(&a, kernel, grid, threads, smem, st, args...);
 }
 
 // ---------------------------------------------------------------------------- group norm
@@ -199,30 +218,26 @@ struct NormArgs {
 };
 
 template <typename T, int V, bool GRAD, int kT>
-void norm_small(const NormPlan& p, const NormArgs& a) {
+cudaError_t norm_small(const NormPlan& p, const NormArgs& a) {
   const auto kernel = norm_small_kernel<T, V, GRAD, kT>;
   static std::atomic<uint64_t> raised{0};
-  if (allow_smem((const void*)kernel, 227 * 1024, raised) != cudaSuccess) return;  // reported by launched()
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.g.n * p.g.splits), (unsigned)p.g.chunks);
-  cfg.blockDim = dim3(kT);
-  cfg.dynamicSmemBytes = p.smem;
-  cfg.stream = a.st;
-  cudaLaunchAttribute cluster[1];
-  cluster[0].id = cudaLaunchAttributeClusterDimension;
-  cluster[0].val.clusterDim.x = (unsigned)p.g.splits;
-  cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
-  cfg.attrs = cluster;
-  cfg.numAttrs = p.g.splits > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<T*>(a.y),
-                     a.mean, a.rstd, a.weight, a.bias, a.dweight, a.dbias, p.cpart ? a.cpart : nullptr, p.g);
+  const cudaError_t e = allow_smem((const void*)kernel, 227 * 1024, raised);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = (unsigned)p.g.splits;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  return launch_with(p.g.splits > 1 ? &cluster : nullptr, kernel,
+                     dim3((unsigned)(p.g.n * p.g.splits), (unsigned)p.g.chunks), kT, p.smem, a.st,
+                     static_cast<const T*>(a.dy), static_cast<const T*>(a.x), static_cast<T*>(a.y), a.mean, a.rstd,
+                     a.weight, a.bias, a.dweight, a.dbias, p.cpart ? a.cpart : nullptr, p.g);
 }
 
 // Floats, rounded up to 16 bytes.
 int ring_at(size_t floats) { return (int)((floats + 3) / 4 * 4); }
 
 template <typename T, int V, int ACT>
-void norm_two_pass(const NormPlan& p, const NormArgs& a) {
+cudaError_t norm_two_pass(const NormPlan& p, const NormArgs& a) {
   NormGeom gs = p.g, ga = p.g;
   const T* x = static_cast<const T*>(a.x);
   constexpr int ring = RowStream<T, V, 1, NORM_THREADS>::kSmem;
@@ -230,17 +245,18 @@ void norm_two_pass(const NormPlan& p, const NormArgs& a) {
   const int smem_s = 4 * (gs.keep + gs.tc * V);                                              // and K
   ga.keep = ring_at(2 * ((size_t)ga.tc * V / ga.cpg + 2));                                   // statistics
   static std::atomic<uint64_t> raised_s{0}, raised_a{0};
-  if (allow_smem((const void*)norm_stats_kernel<T, V>, 113 * 1024, raised_s) != cudaSuccess ||
-      allow_smem((const void*)norm_apply_kernel<T, V, ACT>, 113 * 1024, raised_a) != cudaSuccess)
-    return;  // reported by launched()
+  cudaError_t e = allow_smem((const void*)norm_stats_kernel<T, V>, 113 * 1024, raised_s);
+  if (e == cudaSuccess) e = allow_smem((const void*)norm_apply_kernel<T, V, ACT>, 113 * 1024, raised_a);
+  if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)(gs.n * gs.splits), (unsigned)gs.chunks);
-  norm_stats_kernel<T, V><<<grid, NORM_THREADS, smem_s, a.st>>>(x, a.part, gs);
-  launch_after(norm_apply_kernel<T, V, ACT>, grid, NORM_THREADS, 4 * ga.keep + ring, a.st, x, static_cast<T*>(a.y),
-               a.part, a.mean, a.rstd, a.weight, a.bias, ga);
+  e = launch(norm_stats_kernel<T, V>, grid, NORM_THREADS, smem_s, a.st, x, a.part, gs);
+  if (e != cudaSuccess) return e;
+  return launch_after(norm_apply_kernel<T, V, ACT>, grid, NORM_THREADS, 4 * ga.keep + ring, a.st, x,
+                      static_cast<T*>(a.y), a.part, a.mean, a.rstd, a.weight, a.bias, ga);
 }
 
 template <typename T, int V, int ACT>
-void norm_two_pass_grad(const NormPlan& p, const NormArgs& a) {
+cudaError_t norm_two_pass_grad(const NormPlan& p, const NormArgs& a) {
   NormGeom gs = p.g, ga = p.g;
   const T *x = static_cast<const T*>(a.x), *dy = static_cast<const T*>(a.dy);
   constexpr int ring = RowStream<T, V, 2, NORM_THREADS>::kSmem;
@@ -249,53 +265,43 @@ void norm_two_pass_grad(const NormPlan& p, const NormArgs& a) {
   const int smem_s = 4 * (gs.keep + (int)stat);
   ga.keep = ring_at(2 * stat);
   static std::atomic<uint64_t> raised_s{0}, raised_a{0};
-  if (allow_smem((const void*)norm_grad_sums_kernel<T, V, ACT>, 113 * 1024, raised_s) != cudaSuccess ||
-      allow_smem((const void*)norm_grad_apply_kernel<T, V, ACT>, 113 * 1024, raised_a) != cudaSuccess)
-    return;  // reported by launched()
+  cudaError_t e = allow_smem((const void*)norm_grad_sums_kernel<T, V, ACT>, 113 * 1024, raised_s);
+  if (e == cudaSuccess) e = allow_smem((const void*)norm_grad_apply_kernel<T, V, ACT>, 113 * 1024, raised_a);
+  if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)(gs.n * gs.splits), (unsigned)gs.chunks);
-  norm_grad_sums_kernel<T, V, ACT><<<grid, NORM_THREADS, smem_s, a.st>>>(dy, x, a.mean, a.rstd, a.weight, a.bias,
-                                                                         a.part, a.cpart, gs);
-  launch_after(norm_grad_apply_kernel<T, V, ACT>, grid, NORM_THREADS, 4 * ga.keep + ring, a.st, dy, x,
-               static_cast<T*>(a.y), a.mean, a.rstd, a.weight, a.bias, a.part, ga);
-}
-
-void norm_params(const NormPlan& p, const NormArgs& a) {
-  if (p.cpart && (a.dweight || a.dbias))
-    norm_grad_params_kernel<<<(unsigned)((p.g.c + 31) / 32), 1024, 0, a.st>>>(
-        a.cpart, p.g.n * p.g.splits, p.g.c, a.dweight, a.dbias);
+  e = launch(norm_grad_sums_kernel<T, V, ACT>, grid, NORM_THREADS, smem_s, a.st, dy, x, a.mean, a.rstd, a.weight,
+             a.bias, a.part, a.cpart, gs);
+  if (e != cudaSuccess) return e;
+  return launch_after(norm_grad_apply_kernel<T, V, ACT>, grid, NORM_THREADS, 4 * ga.keep + ring, a.st, dy, x,
+                      static_cast<T*>(a.y), a.mean, a.rstd, a.weight, a.bias, a.part, ga);
 }
 
 template <typename T, int V>
-void norm_forward(const NormPlan& p, const NormArgs& a) {
-  if (p.small)
-    p.threads == 128 ? norm_small<T, V, false, 128>(p, a) : norm_small<T, V, false, 512>(p, a);
-  else if (V * sizeof(T) < 16)
-    norm_two_pass<T, V, ACT_ANY>(p, a);
-  else if (p.g.act == ACT_RELU)
-    norm_two_pass<T, V, ACT_RELU>(p, a);
-  else if (p.g.act == ACT_GELU)
-    norm_two_pass<T, V, ACT_GELU>(p, a);
-  else if (p.g.act == ACT_SILU)
-    norm_two_pass<T, V, ACT_SILU>(p, a);
-  else
-    norm_two_pass<T, V, ACT_NONE>(p, a);
+cudaError_t norm_forward(const NormPlan& p, const NormArgs& a) {
+  if (p.small) return p.threads == 128 ? norm_small<T, V, false, 128>(p, a) : norm_small<T, V, false, 512>(p, a);
+  if (V * sizeof(T) < 16) return norm_two_pass<T, V, ACT_ANY>(p, a);
+  if (p.g.act == ACT_RELU) return norm_two_pass<T, V, ACT_RELU>(p, a);
+  if (p.g.act == ACT_GELU) return norm_two_pass<T, V, ACT_GELU>(p, a);
+  if (p.g.act == ACT_SILU) return norm_two_pass<T, V, ACT_SILU>(p, a);
+  return norm_two_pass<T, V, ACT_NONE>(p, a);
 }
 
 template <typename T, int V>
-void norm_backward(const NormPlan& p, const NormArgs& a) {
-  if (p.small)
-    p.threads == 128 ? norm_small<T, V, true, 128>(p, a) : norm_small<T, V, true, 512>(p, a);
-  else if (V < 4)
-    norm_two_pass_grad<T, V, ACT_ANY>(p, a);
-  else if (p.g.act == ACT_RELU)
-    norm_two_pass_grad<T, V, ACT_RELU>(p, a);
-  else if (p.g.act == ACT_GELU)
-    norm_two_pass_grad<T, V, ACT_GELU>(p, a);
-  else if (p.g.act == ACT_SILU)
-    norm_two_pass_grad<T, V, ACT_SILU>(p, a);
-  else
-    norm_two_pass_grad<T, V, ACT_NONE>(p, a);
-  norm_params(p, a);
+cudaError_t norm_grad_x(const NormPlan& p, const NormArgs& a) {
+  if (p.small) return p.threads == 128 ? norm_small<T, V, true, 128>(p, a) : norm_small<T, V, true, 512>(p, a);
+  if (V < 4) return norm_two_pass_grad<T, V, ACT_ANY>(p, a);
+  if (p.g.act == ACT_RELU) return norm_two_pass_grad<T, V, ACT_RELU>(p, a);
+  if (p.g.act == ACT_GELU) return norm_two_pass_grad<T, V, ACT_GELU>(p, a);
+  if (p.g.act == ACT_SILU) return norm_two_pass_grad<T, V, ACT_SILU>(p, a);
+  return norm_two_pass_grad<T, V, ACT_NONE>(p, a);
+}
+
+template <typename T, int V>
+cudaError_t norm_backward(const NormPlan& p, const NormArgs& a) {
+  const cudaError_t e = norm_grad_x<T, V>(p, a);
+  if (e != cudaSuccess || !p.cpart || !(a.dweight || a.dbias)) return e;
+  return launch(norm_grad_params_kernel, dim3((unsigned)((p.g.c + 31) / 32)), 1024, 0, a.st, a.cpart,
+                p.g.n * p.g.splits, p.g.c, a.dweight, a.dbias);
 }
 
 // ---------------------------------------------------------------------------- attention
@@ -382,29 +388,28 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
 template <typename T, int Boxes, bool Twin>
 int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk, const CUtensorMap& tv,
                    cudaStream_t st) {
+  const char* op = "scb_attention";
   const auto kernel = attn_tc_kernel<T, Boxes, Twin>;
+  const auto join = attn_join_kernel<T>;
   constexpr int smem = AtLayout<Boxes, Twin>::kSmem;
-  static std::atomic<uint64_t> raised{0};
+  static std::atomic<uint64_t> raised{0}, raised_join{0};
   if (!raised.load()) {
     // the kernel's register split draws on what it is launched with: less would wait forever
     cudaFuncAttributes fa;
     const cudaError_t e = cudaFuncGetAttributes(&fa, (const void*)kernel);
-    if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) return finished(op, e);
     if (fa.numRegs != AT_REGS)
       return global_error(SCB_ECUDA, "scb_attention: built with " + std::to_string(fa.numRegs) +
                                          " registers a thread, not " + std::to_string(AT_REGS));
   }
-  const cudaError_t e = allow_smem((const void*)kernel, smem, raised);
-  if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(e));
-  kernel<<<p.grid, AT_THREADS, smem, st>>>(tk, tv, g);
-  if (p.cut || p.twin) {
-    static std::atomic<uint64_t> raised_join{0};
-    const cudaError_t ej = allow_smem((const void*)attn_join_kernel<T>, 128 * 1024, raised_join);
-    if (ej != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_attention: ") + cudaGetErrorString(ej));
-    const dim3 blocks((unsigned)(p.units * (p.unit_rows / 32)));
-    launch_after(attn_join_kernel<T>, blocks, AT_JOIN, (size_t)256 * p.pieces, st, g, p.grid);
-  }
-  return launched("scb_attention");
+  const bool joined = p.cut || p.twin;
+  cudaError_t e = allow_smem((const void*)kernel, smem, raised);
+  if (e == cudaSuccess && joined) e = allow_smem((const void*)join, 128 * 1024, raised_join);
+  if (e == cudaSuccess) e = launch(kernel, dim3((unsigned)p.grid), AT_THREADS, smem, st, tk, tv, g);
+  if (e == cudaSuccess && joined)
+    e = launch_after(join, dim3((unsigned)(p.units * (p.unit_rows / 32))), AT_JOIN, (size_t)256 * p.pieces, st, g,
+                     p.grid);
+  return finished(op, e);
 }
 
 // F<T, V>() for the element type and vector width.
@@ -414,14 +419,11 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
    : vec == 2 ? F<T, 2>(__VA_ARGS__)                                                                         \
               : F<T, 1>(__VA_ARGS__))
 #define NORM_DISPATCH(dtype, vec, F, ...)                                                                    \
-  do {                                                                                                       \
-    if (dtype == SCB_F32)                                                                                    \
-      vec == 4 ? F<float, 4>(__VA_ARGS__) : vec == 2 ? F<float, 2>(__VA_ARGS__) : F<float, 1>(__VA_ARGS__);  \
-    else if (dtype == SCB_F16)                                                                               \
-      NORM_16(__half, vec, F, __VA_ARGS__);                                                                  \
-    else                                                                                                     \
-      NORM_16(__nv_bfloat16, vec, F, __VA_ARGS__);                                                           \
-  } while (0)
+  (dtype == SCB_F16    ? NORM_16(__half, vec, F, __VA_ARGS__)                                                \
+   : dtype == SCB_BF16 ? NORM_16(__nv_bfloat16, vec, F, __VA_ARGS__)                                         \
+   : vec == 4          ? F<float, 4>(__VA_ARGS__)                                                            \
+   : vec == 2          ? F<float, 2>(__VA_ARGS__)                                                            \
+                       : F<float, 1>(__VA_ARGS__))
 
 }  // namespace
 
@@ -471,8 +473,7 @@ int scb_group_norm(const void* x, int64_t x_sn, int64_t x_sl, int dtype, int64_t
     a.x = x; a.y = y; a.mean = mean; a.rstd = rstd; a.weight = weight; a.bias = bias;
     a.part = static_cast<float2*>(work);
     a.st = static_cast<cudaStream_t>(stream);
-    NORM_DISPATCH(dtype, vec, norm_forward, p, a);
-    return launched(op);
+    return finished(op, NORM_DISPATCH(dtype, vec, norm_forward, p, a));
   });
 }
 
@@ -487,9 +488,10 @@ int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const vo
     if (addr(mean) % 4 || addr(rstd) % 4 || addr(weight) % 4 || addr(bias) % 4 || addr(dweight) % 4 || addr(dbias) % 4)
       return refuse(op, "misaligned float pointer");
     if (n == 0 || l == 0) {
-      if (dweight) cudaMemsetAsync(dweight, 0, sizeof(float) * c, st);
-      if (dbias) cudaMemsetAsync(dbias, 0, sizeof(float) * c, st);
-      return launched(op);
+      cudaError_t e = cudaSuccess;
+      if (dweight) e = cudaMemsetAsync(dweight, 0, sizeof(float) * c, st);
+      if (dbias && e == cudaSuccess) e = cudaMemsetAsync(dbias, 0, sizeof(float) * c, st);
+      return finished(op, e);
     }
     if (!dy || !x || !dx || !mean || !rstd) return refuse(op, "NULL data pointer");
     if (d_sn < 0 || d_sl < 0 || x_sn < 0 || x_sl < 0 || !distinct_elements(c, {{l, dx_sl}, {n, dx_sn}}))
@@ -516,8 +518,7 @@ int scb_group_norm_backward(const void* dy, int64_t d_sn, int64_t d_sl, const vo
     a.part = static_cast<float2*>(work);
     a.cpart = a.part + p.part;
     a.st = st;
-    NORM_DISPATCH(dtype, vec, norm_backward, p, a);
-    return launched(op);
+    return finished(op, NORM_DISPATCH(dtype, vec, norm_backward, p, a));
   });
 }
 
@@ -609,13 +610,14 @@ int scb_rotate_axes(const scb_heads* q, const scb_heads* k, int dtype, int64_t b
     if (blocks > kMaxBlocks) return refuse(op, "too many tokens");
     const int smem = g.per_block * g.pairs * (int)sizeof(float2);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const auto launch = [&](auto kernel) { kernel<<<(unsigned)blocks, ROT_THREADS, smem, st>>>(g); };
+    cudaError_t e = cudaSuccess;
+    const auto turn = [&](auto kernel) { e = launch(kernel, dim3((unsigned)blocks), ROT_THREADS, smem, st, g); };
 #define ROT_VECS(T, L)                                        \
   switch (vec) {                                              \
-    case 8: launch(rotary_kernel<T, L, 16 / sizeof(T)>); break; \
-    case 4: launch(rotary_kernel<T, L, 4>); break;            \
-    case 2: launch(rotary_kernel<T, L, 2>); break;            \
-    default: launch(rotary_kernel<T, L, 1>);                  \
+    case 8: turn(rotary_kernel<T, L, 16 / sizeof(T)>); break; \
+    case 4: turn(rotary_kernel<T, L, 4>); break;              \
+    case 2: turn(rotary_kernel<T, L, 2>); break;              \
+    default: turn(rotary_kernel<T, L, 1>);                    \
   }
 #define ROT_LAYOUTS(T)                                              \
   if (layout == ROT_HALF) {                                         \
@@ -634,7 +636,7 @@ int scb_rotate_axes(const scb_heads* q, const scb_heads* k, int dtype, int64_t b
     }
 #undef ROT_LAYOUTS
 #undef ROT_VECS
-    return launched(op);
+    return finished(op, e);
   });
 }
 
@@ -722,11 +724,8 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
     }
     const long blocks = (lq + ATTN_ANY_WARPS - 1) / ATTN_ANY_WARPS;
     if (b > kMaxBlocks / h || blocks > kMaxBlocks / (b * h)) return refuse(op, "too many queries");
-    if (dtype == SCB_F16)
-      attn_any_kernel<__half><<<(unsigned)(blocks * b * h), 32 * ATTN_ANY_WARPS, 0, st>>>(a);
-    else
-      attn_any_kernel<__nv_bfloat16><<<(unsigned)(blocks * b * h), 32 * ATTN_ANY_WARPS, 0, st>>>(a);
-    return launched(op);
+    return finished(op, launch(dtype == SCB_F16 ? attn_any_kernel<__half> : attn_any_kernel<__nv_bfloat16>,
+                               dim3((unsigned)(blocks * b * h)), 32 * ATTN_ANY_WARPS, 0, st, a));
   });
 }
 
@@ -735,10 +734,9 @@ int scb_op_status(void* stream) {
     cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
     unsigned v = 0;
     if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_device_error, sizeof v);
-    if (e != cudaSuccess) return global_error(SCB_ECUDA, std::string("scb_op_status: ") + cudaGetErrorString(e));
-    if (!v) return SCB_OK;
     const unsigned zero = 0;
-    cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
+    if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof zero);
+    if (e != cudaSuccess || !v) return finished("scb_op_status", e);
     return global_error(SCB_EDEVICE,
                         "a kernel gave up on a bounded wait (device error code " + std::to_string(v) + ")");
   });
