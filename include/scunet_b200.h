@@ -379,8 +379,17 @@ int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const
                   float scale, void* work, size_t work_bytes, void* stream);
 
 /* Waits for `stream` and reports a block operator that gave up on a bounded device wait
- * (SCB_EDEVICE; its outputs are undefined) since the last call on this device. */
+ * (SCB_EDEVICE) since the last call on this device: attention on the tensor cores, after a
+ * second, which no input should bring about. The rows that the lost step had a part in are NaN
+ * then. The operators do not wait, so a program calls this where it waits anyway. */
 int scb_op_status(void* stream);
+
+/* For tests: scb_attention whose first CTA leaves out its load number `load` (K and V tiles in
+ * the order of their use), so that its waits run out. */
+int scb_probe_attention_lost(const scb_rows* q, const scb_rows* k, const scb_rows* v, const scb_rows* o, int dtype,
+                             int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, const unsigned char* key_mask,
+                             int64_t mask_sb, float scale, void* work, size_t work_bytes, void* stream,
+                             unsigned load);
 
 #ifdef __cplusplus
 }

@@ -33,7 +33,7 @@ SYMBOLS = [
     "scb_band_sync", "scb_probe_head", "scb_probe_tail", "scb_probe_wait_timeout", "scb_mem_report",
     "scb_profile_report", "scb_check_admission", "scb_profile_kernels",
     "scb_group_norm_workspace", "scb_group_norm", "scb_group_norm_backward", "scb_rotate_axes",
-    "scb_attention_workspace", "scb_attention", "scb_op_status",
+    "scb_attention_workspace", "scb_attention", "scb_op_status", "scb_probe_attention_lost",
 ]
 SCB_OPT_FUSE_TRANS = 1
 SCB_OPT_RESIDUAL32 = 2
@@ -131,6 +131,7 @@ def load_library(path=None):
     lib.scb_attention_workspace.argtypes = [i64, i64, i64, i, i, i, ctypes.POINTER(sz)]
     lib.scb_op_status.argtypes = [vp]
     lib.scb_attention.argtypes = [rows, rows, rows, rows, i, i64, i64, i64, i, i, i, vp, i64, f32, vp, sz, vp]
+    lib.scb_probe_attention_lost.argtypes = [*lib.scb_attention.argtypes, ctypes.c_uint]
     if path is None:
         _lib = lib
     return lib

@@ -61,6 +61,8 @@ constexpr int AT_BOX = AT_KEYS * 128;      // bytes of 128 rows x 64 channels
 // 109 us, two 106 us, five 107 us: the instructions cost what the unit gains).
 constexpr int AT_FMA_PAIRS = 2;
 
+constexpr uint32_t AT_NONE = 0xffffffffu;
+
 struct AttnTcArgs {
   AttnArgs a;
   int share;          // R
@@ -77,6 +79,7 @@ struct AttnTcArgs {
   float* part;        // pieces: [grid][2][d][256] sums, then [grid][2][256] (m c, l)
   float2* part_ml;
   int q_wide, o_wide; // 16-byte accesses to Q and the output allowed
+  uint32_t lose;      // the load that CTA 0 leaves out (scb_probe_attention_lost), else AT_NONE
 };
 
 // Tiles [at_start(cta), at_start(cta + 1)) of the line. Twin units are cut into `cuts` equal
@@ -225,7 +228,8 @@ struct AtPlace {
 };
 
 // A bounded wait that gives up at once when another wait of the CTA has given up. The error
-// word tells the place of the first one that did.
+// word tells the place of the first one that did. `dead` is set before anything that depends on
+// the lost handshake goes on, so whoever writes rows finds it set, and writes NaN.
 enum : unsigned {
   AT_EMPTY = 0x100,
   AT_FULL = 0x200,
@@ -301,19 +305,25 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             if (at.turn) at_wait(empty + at.slot, (at.turn - 1) & 1, dead, AT_EMPTY);
             if (*dead) break;
             mbar_arrive_expect_tx(full + at.slot, L::kTile);
+            if (seq == g.lose && blockIdx.x == 0) continue;
             for (int c = 0; c < Boxes; ++c)
               tma_load_4d(sm + L::kRing + at.slot * L::kTile + c * AT_BOX, w ? &tv : &tk, full + at.slot, 64 * c,
                           (int)(j * AT_KEYS), (g.kv_h >> w & 1) * h, (g.kv_b >> w & 1) * b);
           }
         x += n;
       }
-      // after a wait gave up, loads may still be on their way: none may outlive the CTA
-      if (*dead)
+      // after a wait gave up, loads may still be on their way: none may outlive the CTA. Each
+      // place's last filling is waited for (a wait for one before it, with the same parity as
+      // the filling after, would run out)
+      if (*dead) {
+        uint32_t waited = 0;
         for (uint32_t back = 1; back <= 2 * L::kSlots && back <= seq; ++back) {
-          // (a place that was filled again since passes at once)
           const Place at(seq - back);
+          if (waited >> at.slot & 1) continue;
+          waited |= 1u << at.slot;
           mbar_wait(full + at.slot, at.turn & 1, SCB_ERR_WAIT_ATTN);
         }
+      }
     } else if (warp < 18 && elect_one()) {
       // ---- matrix products of tile t
       const int t = warp - 16;
@@ -592,7 +602,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       }
       *mine = l;
       at_sync(id);
-      l = at_total(half ? *other + l : l + *other);
+      l = *dead ? NAN : at_total(half ? *other + l : l + *other);
       if (!Twin && n == g.tiles) {
         // through the Q tile, whose products are complete: 16-byte chunks of whole rows,
         // `wide` lanes a row, as Q was read

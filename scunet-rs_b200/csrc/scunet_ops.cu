@@ -425,6 +425,83 @@ int attn_tc_launch(const AttnTcArgs& g, const AttnPlan& p, const CUtensorMap& tk
    : vec == 2          ? F<float, 2>(__VA_ARGS__)                                                            \
                        : F<float, 1>(__VA_ARGS__))
 
+// scb_attention; `lose` as in AttnTcArgs.
+int attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const scb_rows* o, int dtype, int64_t b,
+              int64_t lq, int64_t lk, int h, int hk, int d, const unsigned char* key_mask, int64_t mask_sb,
+              float scale, void* work, size_t work_bytes, void* stream, uint32_t lose) {
+  return guarded([&]() -> int {
+    const char* op = "scb_attention";
+    if (dtype != SCB_F16 && dtype != SCB_BF16) return refuse(op, "the element type must be SCB_F16 or SCB_BF16");
+    if (b < 0 || lq < 0 || lk < 0) return refuse(op, "negative size");
+    if (h < 1 || hk < 1 || h % hk)
+      return refuse(op, std::to_string(h) + " query heads cannot share " + std::to_string(hk) + " key heads");
+    if (d < 1 || d > ATTN_ANY_D) return refuse(op, "heads must be 1 to 256 channels wide");
+    if (!q || !k || !v || !o) return refuse(op, "NULL pointer");
+    if (!std::isfinite(scale)) return refuse(op, "the scale must be finite");
+    if (b == 0 || lq == 0) return SCB_OK;
+    if (!q->x || !o->x || (lk && (!k->x || !v->x))) return refuse(op, "NULL data pointer");
+    for (const scb_rows* t : {q, k, v, o}) {
+      if (addr(t->x) % 2) return refuse(op, "data not aligned to its element size");
+      if (t->sb < 0 || t->sl < 0 || t->sh < 0) return refuse(op, "negative strides");
+    }
+    if (!distinct_elements(d, {{b, o->sb}, {lq, o->sl}, {h, o->sh}})) return refuse(op, "overlapping output");
+    if (key_mask && mask_sb < 0) return refuse(op, "negative strides");
+    AttnArgs a{};
+    a.q = q->x; a.k = k->x; a.v = v->x; a.o = o->x;
+    a.mask = key_mask; a.m_sb = mask_sb;
+    a.b = (int)b; a.h = h; a.hk = hk; a.d = d; a.lq = lq; a.lk = lk;
+    a.q_sb = q->sb; a.q_sl = q->sl; a.q_sh = q->sh;
+    a.k_sb = k->sb; a.k_sl = k->sl; a.k_sh = k->sh;
+    a.v_sb = v->sb; a.v_sl = v->sl; a.v_sh = v->sh;
+    a.o_sb = o->sb; a.o_sl = o->sl; a.o_sh = o->sh;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (lk && d <= 128 && attn_tma_ok(*k, b, lk, hk) && attn_tma_ok(*v, b, lk, hk)) {
+      const int sms = sm_count();
+      if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
+      const AttnPlan p = attn_plan(b, lq, lk, h, hk, d, sms);
+      if (p.units <= kMaxBlocks / 256 && p.grid > 0) {
+        if (p.work && (!work || work_bytes < p.work || addr(work) % 16))
+          return refuse(op, "the workspace is too small or not 16-byte aligned (scb_attention_workspace)");
+        AttnTcArgs g{};
+        g.a = a;
+        g.share = p.share; g.rows = p.rows; g.twin = p.twin; g.unit_rows = p.unit_rows; g.cuts = p.cuts;
+        g.row_units = p.row_units;
+        g.units = p.units; g.tiles = p.tiles; g.total = p.total;
+        g.turns = p.rows > 64;  // fewer rows leave the special function units idle anyway
+        g.kv_b = (b > 1 && k->sb ? 1 : 0) | (b > 1 && v->sb ? 2 : 0);
+        g.kv_h = (hk > 1 && k->sh ? 1 : 0) | (hk > 1 && v->sh ? 2 : 0);
+        g.qneg = scale < 0 ? 1 : a.scale_log2 == 0 ? 2 : 0;
+        g.a.scale_log2 = g.qneg == 2 ? 1.f : std::fabs(a.scale_log2);
+        g.lose = lose;
+        g.part = static_cast<float*>(work);
+        g.part_ml = reinterpret_cast<float2*>(g.part + (size_t)p.grid * 2 * 256 * d);
+        const auto wide = [&](const scb_rows* t) {
+          return addr(t->x) % 16 == 0 && t->sb % 8 == 0 && t->sl % 8 == 0 && t->sh % 8 == 0;
+        };
+        g.q_wide = wide(q);
+        g.o_wide = wide(o);
+        CUtensorMap tk, tv;
+        if (!attn_map(&tk, *k, dtype, b, lk, hk, d) || !attn_map(&tv, *v, dtype, b, lk, hk, d))
+          return global_error(SCB_ECUDA, "scb_attention: no tensor map for k or v");
+        const auto boxes = [&](auto type, auto twin) {
+          using T = decltype(type);
+          return d <= 64 ? attn_tc_launch<T, 1, decltype(twin)::value>(g, p, tk, tv, st)
+                         : attn_tc_launch<T, 2, decltype(twin)::value>(g, p, tk, tv, st);
+        };
+        const auto typed = [&](auto type) {
+          return p.twin ? boxes(type, std::true_type{}) : boxes(type, std::false_type{});
+        };
+        return dtype == SCB_F16 ? typed(__half{}) : typed(__nv_bfloat16{});
+      }
+    }
+    const long blocks = (lq + ATTN_ANY_WARPS - 1) / ATTN_ANY_WARPS;
+    if (b > kMaxBlocks / h || blocks > kMaxBlocks / (b * h)) return refuse(op, "too many queries");
+    return finished(op, launch(dtype == SCB_F16 ? attn_any_kernel<__half> : attn_any_kernel<__nv_bfloat16>,
+                               dim3((unsigned)(blocks * b * h)), 32 * ATTN_ANY_WARPS, 0, st, a));
+  });
+}
+
 }  // namespace
 
 extern "C" {
@@ -657,76 +734,14 @@ int scb_attention_workspace(int64_t b, int64_t lq, int64_t lk, int h, int hk, in
 int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const scb_rows* o, int dtype, int64_t b,
                   int64_t lq, int64_t lk, int h, int hk, int d, const unsigned char* key_mask, int64_t mask_sb,
                   float scale, void* work, size_t work_bytes, void* stream) {
-  return guarded([&]() -> int {
-    const char* op = "scb_attention";
-    if (dtype != SCB_F16 && dtype != SCB_BF16) return refuse(op, "the element type must be SCB_F16 or SCB_BF16");
-    if (b < 0 || lq < 0 || lk < 0) return refuse(op, "negative size");
-    if (h < 1 || hk < 1 || h % hk)
-      return refuse(op, std::to_string(h) + " query heads cannot share " + std::to_string(hk) + " key heads");
-    if (d < 1 || d > ATTN_ANY_D) return refuse(op, "heads must be 1 to 256 channels wide");
-    if (!q || !k || !v || !o) return refuse(op, "NULL pointer");
-    if (!std::isfinite(scale)) return refuse(op, "the scale must be finite");
-    if (b == 0 || lq == 0) return SCB_OK;
-    if (!q->x || !o->x || (lk && (!k->x || !v->x))) return refuse(op, "NULL data pointer");
-    for (const scb_rows* t : {q, k, v, o}) {
-      if (addr(t->x) % 2) return refuse(op, "data not aligned to its element size");
-      if (t->sb < 0 || t->sl < 0 || t->sh < 0) return refuse(op, "negative strides");
-    }
-    if (!distinct_elements(d, {{b, o->sb}, {lq, o->sl}, {h, o->sh}})) return refuse(op, "overlapping output");
-    if (key_mask && mask_sb < 0) return refuse(op, "negative strides");
-    AttnArgs a{};
-    a.q = q->x; a.k = k->x; a.v = v->x; a.o = o->x;
-    a.mask = key_mask; a.m_sb = mask_sb;
-    a.b = (int)b; a.h = h; a.hk = hk; a.d = d; a.lq = lq; a.lk = lk;
-    a.q_sb = q->sb; a.q_sl = q->sl; a.q_sh = q->sh;
-    a.k_sb = k->sb; a.k_sl = k->sl; a.k_sh = k->sh;
-    a.v_sb = v->sb; a.v_sl = v->sl; a.v_sh = v->sh;
-    a.o_sb = o->sb; a.o_sl = o->sl; a.o_sh = o->sh;
-    a.scale_log2 = scale * 1.4426950408889634f;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (lk && d <= 128 && attn_tma_ok(*k, b, lk, hk) && attn_tma_ok(*v, b, lk, hk)) {
-      const int sms = sm_count();
-      if (!sms) return global_error(SCB_ECUDA, "no CUDA device");
-      const AttnPlan p = attn_plan(b, lq, lk, h, hk, d, sms);
-      if (p.units <= kMaxBlocks / 256 && p.grid > 0) {
-        if (p.work && (!work || work_bytes < p.work || addr(work) % 16))
-          return refuse(op, "the workspace is too small or not 16-byte aligned (scb_attention_workspace)");
-        AttnTcArgs g{};
-        g.a = a;
-        g.share = p.share; g.rows = p.rows; g.twin = p.twin; g.unit_rows = p.unit_rows; g.cuts = p.cuts;
-        g.row_units = p.row_units;
-        g.units = p.units; g.tiles = p.tiles; g.total = p.total;
-        g.turns = p.rows > 64;  // fewer rows leave the special function units idle anyway
-        g.kv_b = (b > 1 && k->sb ? 1 : 0) | (b > 1 && v->sb ? 2 : 0);
-        g.kv_h = (hk > 1 && k->sh ? 1 : 0) | (hk > 1 && v->sh ? 2 : 0);
-        g.qneg = scale < 0 ? 1 : a.scale_log2 == 0 ? 2 : 0;
-        g.a.scale_log2 = g.qneg == 2 ? 1.f : std::fabs(a.scale_log2);
-        g.part = static_cast<float*>(work);
-        g.part_ml = reinterpret_cast<float2*>(g.part + (size_t)p.grid * 2 * 256 * d);
-        const auto wide = [&](const scb_rows* t) {
-          return addr(t->x) % 16 == 0 && t->sb % 8 == 0 && t->sl % 8 == 0 && t->sh % 8 == 0;
-        };
-        g.q_wide = wide(q);
-        g.o_wide = wide(o);
-        CUtensorMap tk, tv;
-        if (!attn_map(&tk, *k, dtype, b, lk, hk, d) || !attn_map(&tv, *v, dtype, b, lk, hk, d))
-          return global_error(SCB_ECUDA, "scb_attention: no tensor map for k or v");
-        const auto boxes = [&](auto type, auto twin) {
-          using T = decltype(type);
-          return d <= 64 ? attn_tc_launch<T, 1, decltype(twin)::value>(g, p, tk, tv, st)
-                         : attn_tc_launch<T, 2, decltype(twin)::value>(g, p, tk, tv, st);
-        };
-        const auto typed = [&](auto type) {
-          return p.twin ? boxes(type, std::true_type{}) : boxes(type, std::false_type{});
-        };
-        return dtype == SCB_F16 ? typed(__half{}) : typed(__nv_bfloat16{});
-      }
-    }
-    const long blocks = (lq + ATTN_ANY_WARPS - 1) / ATTN_ANY_WARPS;
-    if (b > kMaxBlocks / h || blocks > kMaxBlocks / (b * h)) return refuse(op, "too many queries");
-    return finished(op, launch(dtype == SCB_F16 ? attn_any_kernel<__half> : attn_any_kernel<__nv_bfloat16>,
-                               dim3((unsigned)(blocks * b * h)), 32 * ATTN_ANY_WARPS, 0, st, a));
-  });
+  return attention(q, k, v, o, dtype, b, lq, lk, h, hk, d, key_mask, mask_sb, scale, work, work_bytes, stream, AT_NONE);
+}
+
+int scb_probe_attention_lost(const scb_rows* q, const scb_rows* k, const scb_rows* v, const scb_rows* o, int dtype,
+                             int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, const unsigned char* key_mask,
+                             int64_t mask_sb, float scale, void* work, size_t work_bytes, void* stream,
+                             unsigned load) {
+  return attention(q, k, v, o, dtype, b, lq, lk, h, hk, d, key_mask, mask_sb, scale, work, work_bytes, stream, load);
 }
 
 int scb_op_status(void* stream) {

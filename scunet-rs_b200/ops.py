@@ -272,7 +272,8 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
     q is [b, lq, h, d], k and v [b, lk, hk, d] with d at most 256; query head i reads key head
     i / (h / hk). key_mask is bool or uint8 [b, lk], nonzero = visible: what hidden keys hold
     does not matter, and queries with no visible key give zeros. scale defaults to
-    1 / sqrt(d). Forward only: there is no gradient. Fast (tensor cores) for d up to 128 and 16-byte aligned rows of k and v."""
+    1 / sqrt(d). Forward only: there is no gradient. A lost wait on the device makes the rows it
+    had a part in NaN; `status` tells. Fast (tensor cores) for d up to 128 and 16-byte aligned rows of k and v."""
     dt = _dtype(q, "q")
     if _recording():
         _no_gradient("attention has no gradient", q, k, v, out)
@@ -306,7 +307,8 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
 
 def status(stream=None):
     """Wait for the stream (default: the current one) and raise if an operator's kernel gave up
-    on a bounded wait since the last call; its outputs are undefined then."""
+    on a bounded wait since the last call. The operators themselves do not wait: call this where
+    the program waits anyway."""
     stream = stream or torch.cuda.current_stream()
     with torch.cuda.device(stream.device):
         if _library().scb_op_status(stream.cuda_stream) != 0:
