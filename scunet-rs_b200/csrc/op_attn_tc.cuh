@@ -182,10 +182,11 @@ struct AtLayout {
   // Where P_t lies: beside S_t in TMEM for heads up to 64 wide; in shared memory for wider
   // ones, where S and O fill TMEM, at the price of two ring slots (8160 x 8160 x 8 x 128: 293
   // us over S_t, 272 us so; where every key is read from DRAM for 256 rows only, 159 and 179
-  // us); over S_t with Twin, whose tiles need the slots
+  // us); over S_t with Twin, whose tiles need two slots each
   static constexpr bool kSharedP = Boxes == 2 && !Twin;
   static constexpr bool kOwnP = Boxes == 1 || kSharedP;
-  static constexpr int kSlots = Boxes == 1 ? 10 : kSharedP ? 3 : 5;
+  static constexpr int kSlots = Boxes == 1 ? 10 : kSharedP ? 3 : 4;
+  static_assert(!Twin || kSlots % 2 == 0, "each tile of Twin has half of the ring");
   static constexpr int kQ = 0;
   static constexpr int kPTile = 2 * AT_BOX;               // 128 rows x 128 keys
   static constexpr int kSharedPAt = 2 * kTile;
