@@ -76,7 +76,8 @@ struct AttnTcArgs {
   long total;         // units * tiles
   int kv_b, kv_h;     // 1 where K / V differ by picture / head (0: broadcast), bit 0 K, bit 1 V
   int qneg;           // the scale is negative (Q is negated) or, 2, zero (Q is cleared)
-  float* part;        // pieces: [grid][2][d][256] sums, then [grid][2][256] (m c, l)
+  float* part;        // pieces, two of a CTA (its first and last unit), one with twin:
+                      // [pieces][d][256] sums, then [pieces][256] (m c, l)
   float2* part_ml;
   int q_wide, o_wide; // 16-byte accesses to Q and the output allowed
   uint32_t lose;      // the load that CTA 0 leaves out (scb_probe_attention_lost), else AT_NONE
@@ -635,7 +636,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
       } else {
         // the piece is kept channel by channel, so that a warp stores 32 rows side by side
-        const long piece = 2L * blockIdx.x + (x == x0 ? 0 : 1);
+        const long piece = Twin ? (long)blockIdx.x : 2L * blockIdx.x + (x == x0 ? 0 : 1);
         const int col = Twin ? 128 * t + unit_row : unit_row;
         if (half == 0) g.part_ml[piece * 256 + col] = make_float2(m == -INFINITY ? m : fmaxf(m * c, AT_LOWEST), l);
         float* o = g.part + piece * 256 * d + col;
@@ -684,9 +685,9 @@ __global__ void __launch_bounds__(AT_JOIN) attn_join_kernel(const __grid_constan
   if (c0 == c1 && !g.twin) return;  // written by its CTA
   const int pieces = g.twin ? 2 * g.cuts : (int)(c1 - c0 + 1);
   // piece i: its place among all, in rows; only the first can be its CTA's second
-  const long first = g.twin ? 2 * unit : 2 * c0 + (at_start(g, c0, grid) >= t0 ? 0 : 1);
+  const long first = 2 * c0 + (at_start(g, c0, grid) >= t0 ? 0 : 1);
   const auto place = [&](int i) -> long {
-    return g.twin ? 2 * (unit + g.units * (i >> 1)) : i == 0 ? first : 2 * (c0 + i);
+    return g.twin ? unit + g.units * (i >> 1) : i == 0 ? first : 2 * (c0 + i);
   };
   const auto column = [&](int i) { return (g.twin ? 128 * (i & 1) : 0) + row0 + lane; };
   float *ms = join_sm, *ls = join_sm + 32 * pieces;

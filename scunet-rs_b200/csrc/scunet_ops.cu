@@ -350,7 +350,7 @@ struct AttnPlan {
   long rows, row_units, units, tiles, total;
   int grid, cuts, pieces;  // pieces: of a unit, at most
   bool cut;
-  size_t work;
+  size_t places, work;  // pieces of all units (places for them), the workspace's bytes
 };
 AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int sms) {
   AttnPlan p{};
@@ -381,7 +381,8 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
   p.grid = (int)(grid < kMaxBlocks ? grid : kMaxBlocks);
   p.cut = p.grid != p.units;
   p.pieces = p.twin ? 2 * p.cuts : (int)(p.grid / p.units + 2);
-  p.work = p.cut || p.twin ? (size_t)p.grid * 2 * 256 * (d + 2) * sizeof(float) : 0;
+  p.places = p.twin ? p.grid : p.cut ? 2 * (size_t)p.grid : 0;
+  p.work = p.places * 256 * (d + 2) * sizeof(float);
   return p;
 }
 
@@ -475,7 +476,7 @@ int attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const scb
         g.a.scale_log2 = g.qneg == 2 ? 1.f : std::fabs(a.scale_log2);
         g.lose = lose;
         g.part = static_cast<float*>(work);
-        g.part_ml = reinterpret_cast<float2*>(g.part + (size_t)p.grid * 2 * 256 * d);
+        g.part_ml = reinterpret_cast<float2*>(g.part + p.places * 256 * d);
         const auto wide = [&](const scb_rows* t) {
           return addr(t->x) % 16 == 0 && t->sb % 8 == 0 && t->sl % 8 == 0 && t->sh % 8 == 0;
         };
