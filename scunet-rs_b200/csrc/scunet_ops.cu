@@ -357,9 +357,15 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
   p.share = h / hk;
   p.rows = lq * p.share;
   p.tiles = (lk + AT_KEYS - 1) / AT_KEYS;
-  // (twin units always leave pieces, so not for more units than a few rounds of CTAs: the
-  // workspace stays below 160 MB)
-  p.twin = p.rows <= 128 && p.tiles > 1 && b * hk <= 4L * sms;
+  // Twin units always leave pieces, whose cost grows with the rows, so they need some tiles.
+  // Heads of 64 fp16, us without and with twin:
+  //   140 pictures x 8 rows, 500 keys: 17 / 21; 1000 keys: 35 / 24; 128 rows, 1000 keys: 39 / 30
+  //   2000 x 8, 300: 156 / 158; 500: 175 / 159; 2040: 413 / 275;  2000 x 128, 1000: 301 / 352; 2040: 462 / 448
+  // and with very few units the join of many pieces of each (4 x 1 row, 32640 keys: 56 / 65;
+  // 16 x 1: 69 / 54). Past a GB of workspace the units are whole, without any.
+  const long keys_of_heads = b * hk, least = keys_of_heads <= sms ? 5 : p.rows <= 32 ? 4 : p.rows / 8;
+  p.twin = p.rows <= 128 && p.tiles >= least && keys_of_heads >= 8 &&
+           (keys_of_heads <= sms || keys_of_heads <= (1L << 30) / (256 * (d + 2) * (long)sizeof(float)));
   p.unit_rows = p.twin ? 128 : 256;
   p.row_units = (p.rows + p.unit_rows - 1) / p.unit_rows;
   p.units = b * hk * p.row_units;
@@ -368,9 +374,9 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
   const long waves = (p.units + sms - 1) / sms;
   if (p.twin) {
     // as many pieces as one round of CTAs holds (a second round measured 50 % slower), each
-    // of two tiles or more
-    const long most = p.tiles / 2, s = sms / p.units;
-    p.cuts = (int)(s < 1 ? 1 : s < most ? s : most);
+    // of eight tiles or more (16 pictures x 1 row, 2040 keys: 29 us from two tiles on, 22 so)
+    const long most = p.tiles / 8, s = sms / p.units;
+    p.cuts = (int)std::max(1L, std::min(s, most));
     grid = p.units * p.cuts;
   } else if (p.units < sms) {
     const long most = p.total / 4;  // at least four tiles a CTA

@@ -13,6 +13,8 @@ LOST = {
     "whole units, the first keys": ((2, 300, 300, 2, 2, 64), 0, (0, slice(0, 256), 0)),
     "whole units, the last values": ((2, 300, 300, 2, 2, 32), 5, (0, slice(0, 256), 0)),
     "cut units": ((1, 300, 1025, 1, 1, 128), 3, (0, slice(0, 256), 0)),
+    "few rows, eight units": ((2, 1, 3000, 4, 4, 64), 2, (0, 0, 0)),
+    "few rows, eight units, shared heads, wide": ((2, 3, 1025, 8, 4, 128), 1, (0, slice(0, 3), slice(0, 2))),
     "few rows": ((2, 1, 3000, 2, 2, 64), 2, (0, 0, 0)),
     "few rows, wide": ((1, 3, 1025, 2, 2, 128), 1, (0, slice(0, 3), 0)),
 }

@@ -10,6 +10,9 @@ from test_ops_gpu import check_attention, ops, qkv_of, torch  # noqa: F401 (fixt
 pytestmark = pytest.mark.gpu
 
 CUTS = {  # b, lq, lk, h, hk, d
+    "few rows, eight units": (2, 1, 3000, 4, 4, 64),
+    "few rows, eight units, shared heads, wide": (2, 3, 1025, 8, 4, 128),
+    "few rows, many pictures": (160, 2, 500, 1, 1, 32),
     "few rows": (2, 1, 3000, 2, 2, 64),
     "few rows, shared heads, wide": (1, 3, 1025, 4, 2, 128),
     "few rows, one piece a tile": (2, 2, 257, 1, 1, 32),
