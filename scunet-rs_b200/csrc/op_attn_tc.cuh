@@ -56,11 +56,6 @@ constexpr float AT_LIFT = __is_same(T, __half) ? 7.f : 0.f;
 constexpr float AT_LOWEST = -FLT_MAX;      // m of visible scores that are all -inf
 constexpr int AT_BOX = AT_KEYS * 128;      // bytes of 128 rows x 64 channels
 
-// Of every 16 pairs of weights, those whose 2^y is computed by exp2_pair on the FMA units
-// instead of the special function unit (256 rows x 8192 keys, heads of 64, on every SM: none
-// 109 us, two 106 us, five 107 us: the instructions cost what the unit gains).
-constexpr int AT_FMA_PAIRS = 2;
-
 constexpr uint32_t AT_NONE = 0xffffffffu;
 
 struct AttnTcArgs {
@@ -112,38 +107,6 @@ template <>
 __device__ __forceinline__ uint32_t at_pack<__nv_bfloat16>(float a, float b) {
   __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
-}
-
-// 2^y of two values y <= 15 on the FMA units: y = n + f, n the nearest integer (it appears in
-// the low bits of y + 1.5 2^23), |f| <= 1/2; 2^f by the cubic of least relative error on that
-// interval (fitted by linear programming: 7.5e-5 at most, 5.2e-5 rms, where rounding the
-// weight to fp16 adds 2e-4 rms and to bf16 1.6e-3). For fp16 n is added to the exponent: y
-// stops at -126, whose 2^-126 is a weight of 0 in fp16 and nothing in the float32 sum; NaN
-// gives NaN or the largest float, which at_total finds in the sum. In bf16 2^-126 would count
-// where a value is large, so there the cubic is multiplied by 2^n, whose bits (n + 127) << 23
-// are zero at n = -127, where y stops.
-template <typename T>
-__device__ __forceinline__ float2 exp2_pair(float2 y) {
-  constexpr bool kZero = __is_same(T, __nv_bfloat16);
-  constexpr float kLeast = kZero ? -127.f : -126.f;
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.x) : "f"(kLeast));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y.y) : "f"(kLeast));
-  const float2 z = __fadd2_rn(y, make_float2(12582912.f, 12582912.f));
-  const float2 n = __fadd2_rn(z, make_float2(-12582912.f, -12582912.f));
-  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), y);
-  float2 p = __ffma2_rn(f, make_float2(0.0551714189f, 0.0551714189f), make_float2(0.24261117f, 0.24261117f));
-  p = __ffma2_rn(p, f, make_float2(0.693261027f, 0.693261027f));
-  p = __ffma2_rn(p, f, make_float2(0.999928057f, 0.999928057f));
-  // (z << 23) + the bits of p, or of 1, as one multiply-add
-  int rx, ry;
-  asm("mad.lo.s32 %0, %1, 8388608, %2;"
-      : "=r"(rx)
-      : "r"(__float_as_int(z.x)), "r"(kZero ? 127 << 23 : __float_as_int(p.x)));
-  asm("mad.lo.s32 %0, %1, 8388608, %2;"
-      : "=r"(ry)
-      : "r"(__float_as_int(z.y)), "r"(kZero ? 127 << 23 : __float_as_int(p.y)));
-  const float2 r = make_float2(__int_as_float(rx), __int_as_float(ry));
-  return kZero ? __fmul2_rn(p, r) : r;
 }
 
 // 1 / l of a row's final sum: 0 when no key was visible, NaN when nothing was above -inf.
@@ -570,8 +533,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           for (int e = 0; e < 16; ++e) {
             const float2 y = __ffma2_rn(make_float2(s[32 * i + 2 * e], s[32 * i + 2 * e + 1]), make_float2(c, c),
                                         make_float2(mc, mc));
-            const float2 v = (e * AT_FMA_PAIRS) % 16 < AT_FMA_PAIRS ? exp2_pair<T>(y)
-                                                                    : make_float2(ex2_approx(y.x), ex2_approx(y.y));
+            const float2 v = make_float2(ex2_approx(y.x), ex2_approx(y.y));
             sum[e & 1] = __fadd2_rn(sum[e & 1], v);
             p[e] = at_pack<T>(v.x, v.y);
           }
