@@ -371,9 +371,10 @@ int scb_attention_workspace(int64_t b, int64_t lq, int64_t lk, int h, int hk, in
  * [b][lk][hk][d] in SCB_F16 or SCB_BF16, d at most 256; query head i reads key head
  * i / (h / hk). key_mask (NULL: all visible) is bytes [b][lk], rows mask_sb apart, 0 =
  * hidden: a hidden key's values do not matter, NaN and infinities included. Queries with no
- * visible key give zeros. Heads up to 128 wide whose k and v have 16-byte aligned rows run on
- * the tensor cores, their weights rounded to the operands' type once; others on a general
- * kernel that is slower by two orders of magnitude on long inputs. */
+ * visible key give zeros; those whose visible scores are all -inf, or any of them NaN or +inf,
+ * NaN. Heads up to 128 wide whose k and v have 16-byte aligned rows run on the tensor cores,
+ * their weights rounded to the operands' type once; others on a general kernel that is slower by
+ * two orders of magnitude on long inputs. */
 int scb_attention(const scb_rows* q, const scb_rows* k, const scb_rows* v, const scb_rows* o, int dtype, int64_t b,
                   int64_t lq, int64_t lk, int h, int hk, int d, const unsigned char* key_mask, int64_t mask_sb,
                   float scale, void* work, size_t work_bytes, void* stream);

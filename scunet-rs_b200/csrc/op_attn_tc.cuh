@@ -28,15 +28,18 @@
 // tell rows that see nothing (zeros) from rows whose visible scores are all -inf (0 / 0, NaN):
 // the weights of any other row sum up to 1 or more.
 //
-// Precision: scores, maxima, sums and O are float32; the weights are rounded to the
-// operands' type for P V, which makes the result's error 1.4 times that of its own rounding.
+// Precision: scores, maxima, sums and O are float32, exponentials those of the special function
+// unit (2 ulp); the weights are rounded to the operands' type for P V, which the tensor cores
+// want alike, and which makes the result's error 1.4 times that of its own rounding.
 //
 // Bound: the softmax. A pair of 128 x 128 tiles takes 2048 cycles of the special function
 // units (the softmax alone, without products or waits, measured 2190 with 16 warps and 2712
-// with 8) and about 2900 here, 1300 to 2050 of them on the tensor cores. 8160 queries and
-// keys, 8 heads of 128 bf16: 300 us (909 TFLOP/s); 4 x 2040 x 2040, 16 heads of 32 fp16:
-// 123 us. One query over 32640 keys, 2 x 16 heads of 64: 68 us (3.9 TB/s), where what is left
-// is the start, the pieces and their join.
+// with 8) and 2830 here with heads up to 64; 3270 with heads of 128 whose keys come from L2,
+// 4060 from DRAM (2048 of them products). Between two units of a CTA 5000 to 6000 cycles pass
+// without either (heads of 32), 15000 with heads of 128, and the join of cut units adds 11 to 28
+// us. 4 x 2040 x 2040, 16 heads of 32 fp16: 121 us. 8160 queries and keys, 8 heads of 128 bf16:
+// 267 us at 1.9 GHz, 297 us where the power limit holds the clock at 1.7 (918 TFLOP/s). One query
+// over 32640 keys, 2 x 16 heads of 64 fp16: 66 us (4.1 TB/s), 12 of them the join.
 #pragma once
 #include <cfloat>
 
@@ -144,9 +147,9 @@ template <int Boxes, bool Twin>
 struct AtLayout {
   static constexpr int kTile = Boxes * AT_BOX;            // one Q, K or V tile
   // Where P_t lies: beside S_t in TMEM for heads up to 64 wide; in shared memory for wider
-  // ones, where S and O fill TMEM, at the price of two ring slots (8160 x 8160 x 8 x 128: 293
-  // us over S_t, 272 us so; where every key is read from DRAM for 256 rows only, 159 and 179
-  // us); over S_t with Twin, whose tiles need two slots each
+  // ones, where S and O fill TMEM, at the price of two ring slots (8160 x 8160 x 8 x 128 in
+  // short runs: 293 us over S_t, 272 us so when it came in; where every key is read from DRAM for
+  // 256 rows only, 159 and 179 us); over S_t with Twin, whose tiles need two slots each
   static constexpr bool kSharedP = Boxes == 2 && !Twin;
   static constexpr bool kOwnP = Boxes == 1 || kSharedP;
   static constexpr int kSlots = Boxes == 1 ? 10 : kSharedP ? 3 : 4;

@@ -271,9 +271,10 @@ def attention(q, k, v, *, scale=None, key_mask=None, out=None):
 
     q is [b, lq, h, d], k and v [b, lk, hk, d] with d at most 256; query head i reads key head
     i / (h / hk). key_mask is bool or uint8 [b, lk], nonzero = visible: what hidden keys hold
-    does not matter, and queries with no visible key give zeros. scale defaults to
-    1 / sqrt(d). Forward only: there is no gradient. A lost wait on the device makes the rows it
-    had a part in NaN; `status` tells. Fast (tensor cores) for d up to 128 and 16-byte aligned rows of k and v."""
+    does not matter, and queries with no visible key give zeros (with nothing but scores of -inf
+    NaN, as 0 / 0 is). scale defaults to 1 / sqrt(d). Fast (tensor cores) for d up to 128 and
+    16-byte aligned rows of k and v. Forward only: there is no gradient. A lost wait on the device
+    makes the rows it had a part in NaN; `status` tells."""
     dt = _dtype(q, "q")
     if _recording():
         _no_gradient("attention has no gradient", q, k, v, out)
