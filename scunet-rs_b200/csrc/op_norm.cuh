@@ -306,7 +306,8 @@ __device__ __forceinline__ float2 group_moments(const BlockSums<V, T>& s, const 
     sq += v.y;
   }
   m2 = warp_sum(m2);
-  far = far || warp_sum(sq) > NORM_FAR * m2;
+  sq = warp_sum(sq);
+  far |= sq > NORM_FAR * m2;
   return make_float2(mean, m2);
 }
 
