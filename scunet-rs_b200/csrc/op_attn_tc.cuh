@@ -645,9 +645,13 @@ __global__ void __launch_bounds__(AT_JOIN) attn_join_kernel(const __grid_constan
   const long unit = blockIdx.x / groups;
   const int row0 = (int)(blockIdx.x - unit * groups) * 32;
   const long bh = unit / g.row_units, r0 = (unit - bh * g.row_units) * g.unit_rows + row0;
-  if (r0 >= g.rows) return;
   const long t0 = unit * g.tiles, c0 = at_owner(g, t0, grid), c1 = at_owner(g, t0 + g.tiles - 1, grid);
-  if (c0 == c1 && !g.twin) return;  // written by its CTA
+  if (r0 >= g.rows || (c0 == c1 && !g.twin)) {  // no rows, or written by their CTA
+    // every block waits: a grid that ended without it would let the stream's next kernel start
+    // before the main kernel's rows are written
+    wait_for_previous();
+    return;
+  }
   const int pieces = g.twin ? 2 * g.cuts : (int)(c1 - c0 + 1);
   // piece i: its place among all, in rows; only the first can be its CTA's second
   const long first = 2 * c0 + (at_start(g, c0, grid) >= t0 ? 0 : 1);

@@ -385,7 +385,7 @@ AttnPlan attn_plan(int64_t b, int64_t lq, int64_t lk, int h, int hk, int d, int 
     grid = sms;
   }
   p.grid = (int)(grid < kMaxBlocks ? grid : kMaxBlocks);
-  p.cut = p.grid != p.units;
+  p.cut = p.grid != p.units && p.tiles > 1;  // units of one tile are whole wherever the ranges end
   p.pieces = p.twin ? 2 * p.cuts : (int)(p.grid / p.units + 2);
   p.places = p.twin ? p.grid : p.cut ? 2 * (size_t)p.grid : 0;
   p.work = p.places * 256 * (d + 2) * sizeof(float);

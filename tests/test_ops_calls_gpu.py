@@ -3,7 +3,7 @@ import ctypes
 
 import pytest
 
-from test_ops_gpu import ops, torch  # noqa: F401 (fixtures)
+from test_ops_gpu import check_attention, ops, qkv_of, torch  # noqa: F401 (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,20 @@ def test_few_row_workspace_is_what_is_written(torch, ops):  # noqa: F811
     want = torch.softmax(torch.einsum("bqhd,bkhd->bhqk", q.double(), k.double()) * 128 ** -0.5, 3)
     want = torch.einsum("bhqk,bkhd->bqhd", want, k.double())
     assert (ops.attention(q, k, k).double() - want).abs().max() < 4 * 2.0 ** -11 * 5  # |k| up to 5
+
+
+@pytest.mark.parametrize("heads,lq,lk,d", [(200, 256, 128, 128), (200, 256, 40, 64), (1200, 1, 100, 16),
+                                           (216, 250, 300, 64)])
+def test_next_kernel_sees_every_row(torch, ops, heads, lq, lk, d):  # noqa: F811
+    """What the stream runs after attention starts when all its rows are there, also where units
+    outnumber the CTAs and none is cut."""
+    q, k, v = qkv_of(torch, 1, lq, lk, heads, heads, d, torch.float16, seed=95)
+    for _ in range(20):
+        out = torch.zeros_like(q)
+        ops.attention(q, k, v, out=out)
+        then = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(then, out)
+    check_attention(torch, ops, q, k, v, got=then)
+    if lk <= 128:  # whole units leave no pieces
+        assert ops._work_bytes("scb_attention_workspace", 0, 1, lq, lk, heads, heads, d) == 0
